@@ -25,6 +25,11 @@ extern "C" {
 #define TB_ELAUNCH (-3)  /* the CUDA launch (or a CUDA runtime call) failed         */
 #define TB_EDEVICE (-4)  /* the current device is not sm_100 / has no usable kernel */
 
+/* Element types of the entry points that take more than one (`*_type` arguments). */
+#define TB_FP16 0
+#define TB_BF16 1
+#define TB_FP32 2
+
 /* Text of the last error reported on this host thread ("" when none). */
 const char *tb_last_error(void);
 
@@ -449,8 +454,8 @@ int tb_head_merge(const float *part, const int64_t *part_idx, const int64_t *tar
 int tb_embed_rows(const int64_t *ids, const int64_t *pos_idx, const uint16_t *table, float *out,
                   int64_t rows, int64_t hidden, int64_t vocab, void *stream);
 
-/* Token ids tb_embed_rows found outside [0, vocab) since the library was loaded (-1 when the
- * counter cannot be read). */
+/* Token ids tb_embed_rows and tb_embedding_fwd found outside [0, vocab) since the library was
+ * loaded (-1 when a counter cannot be read). */
 int64_t tb_embed_invalid_ids(void);
 
 int tb_head_order(const int64_t *targets, int64_t rows, int64_t ignore_index, int64_t *order,
@@ -543,6 +548,99 @@ int64_t tb_head_dh_workspace(int64_t rows, int64_t cols, int64_t hidden_dim);
  * logits <- fp16((exp(z - lse[row]) - [col == target]) * grad_scale); unlabelled rows untouched. */
 int tb_head_dlogits(uint16_t *logits, const int64_t *targets, const float *lse, int64_t rows,
                     int64_t cols, int64_t ld, int64_t col_offset, float grad_scale, void *stream);
+
+/* Dropout from a counter-based generator: y[i] = residual[i] + (w_i >= threshold ? x[i] * scale
+ * : 0) for n elements; residual (y's type) may be NULL. w_i is word i % 4 of Philox4x32-10 at
+ * counter offset + i / 4 under the 64-bit key `seed`; threshold 0 .. 2^32 (2^32 drops all). With
+ * `state` (device int64 [2]: seed, offset) the key is state[0] and state[1] is added to offset,
+ * read when the kernel runs; `used` (device int64 [2], may be NULL) receives the seed and offset
+ * used. The backward is the same call over dy. x_type and y_type: equal, or one of them TB_FP32.
+ * Buffers aligned to their elements (16 bytes takes the vector path). The reference's dropout is
+ * PyTorch's, with a stored mask (solution/model.py:195-206). */
+int tb_dropout(const void *x, int32_t x_type, const void *residual, void *y, int32_t y_type,
+               int64_t n, int64_t threshold, float scale, int64_t seed, int64_t offset,
+               const int64_t *state, int64_t *used, void *stream);
+
+/* Per-head RMS norms of queries and keys, the LoRA add and the rotation in one pass, token-major
+ * (tb_rope_tokens_fwd with head norms; solution/rope.py:24-75). qkv [rows, (n_heads + 2 n_kv) *
+ * head_dim] with ld elements between rows, in `type`; lora_q / lora_v contiguous in lora_type (may
+ * be NULL); x = qkv + lora in fp32, q and k rows become x * rsqrt(mean(x^2) + eps) *
+ * (weight_offset + weight) (a NULL weight: 1), turned on their first `rot` dims by row
+ * pos_idx[token] % seq of cos / sin (fp32 [seq, rot]); v = x. q [rows, n_heads, head_dim], k and
+ * v [rows, n_kv, head_dim] in `type`. A token whose position is outside [0, batch * seq) gives
+ * zero rows. head_dim (at most 4096) and rot even; multiples of 16 with 16-byte aligned buffers
+ * take the vector path. */
+int tb_norm_rope_fwd(const void *qkv, int32_t type, int64_t ld, const void *lora_q,
+                     const void *lora_v, int32_t lora_type, const void *q_weight,
+                     const void *k_weight, int32_t weight_type, float weight_offset, float eps,
+                     const float *cos, const float *sin, int32_t rot, const int64_t *pos_idx,
+                     void *q, void *k, void *v, int64_t rows, int64_t batch, int64_t seq,
+                     int32_t n_heads, int32_t n_kv, int32_t head_dim, void *stream);
+
+/* Its backward (solution/rope.py:78-128 with the norms): dqkv [rows, (n_heads + 2 n_kv) *
+ * head_dim] contiguous, from dq, dk, dv (each may be NULL: zero) and the forward's inputs; and,
+ * when dq_weight / dk_weight are given, the weights' gradients (weight_type), whose fp32 sums over
+ * token ranges go to `workspace` (tb_norm_rope_bwd_workspace bytes) and are added in a fixed
+ * order. Outside positions give zero rows. */
+int tb_norm_rope_bwd(const void *dq, const void *dk, const void *dv, const void *qkv, int32_t type,
+                     int64_t ld, const void *lora_q, int32_t lora_type, const void *q_weight,
+                     const void *k_weight, int32_t weight_type, float weight_offset, float eps,
+                     const float *cos, const float *sin, int32_t rot, const int64_t *pos_idx,
+                     void *dqkv, void *dq_weight, void *dk_weight, void *workspace,
+                     int64_t workspace_bytes, int64_t rows, int64_t batch, int64_t seq,
+                     int32_t n_heads, int32_t n_kv, int32_t head_dim, void *stream);
+
+/* Bytes of workspace tb_norm_rope_bwd needs for the weights' gradients on the current device. */
+int64_t tb_norm_rope_bwd_workspace(int64_t rows, int32_t head_dim);
+
+/* Scaled embedding: out[t] = scale * table[ids[t]] for n ids (int64, or int32 when ids_int64 is 0);
+ * table rows `ld` elements apart, in `type`; out [n, hidden] in `type` or TB_FP32, rounded once.
+ * An id outside [0, vocab) reads nothing: its row is zeros and it is counted
+ * (tb_embed_invalid_ids). Beside tb_embed_rows (solution/model.py:220-225). */
+int tb_embedding_fwd(const void *ids, int32_t ids_int64, const void *table, int32_t type,
+                     int64_t ld, void *out, int32_t out_type, float scale, int64_t n,
+                     int64_t hidden, int64_t vocab, void *stream);
+
+/* Its gradient: dw[v] = scale * sum of dy[t] over the tokens t with ids[t] == v, 0 for ids without
+ * tokens, contiguous [vocab, hidden] in `type`; with `accumulate` the sums are added to what dw
+ * holds and rows of other ids are left alone. Ids outside [0, vocab) and `padding_idx` (-1: none)
+ * give nothing. fp32 sums in a fixed order (the tokens sorted by id, then position), rounded once.
+ * dy [n, hidden] in `type`, or TB_FP32, or any type when `type` is TB_FP32. `workspace`:
+ * tb_embedding_grad_workspace bytes, 16-byte aligned. */
+int tb_embedding_grad(const void *ids, int32_t ids_int64, const void *dy, int32_t dy_type, void *dw,
+                      int32_t type, float scale, int64_t padding_idx, int32_t accumulate,
+                      int64_t n, int64_t hidden, int64_t vocab, void *workspace,
+                      int64_t workspace_bytes, void *stream);
+
+/* Bytes of workspace tb_embedding_grad needs. */
+int64_t tb_embedding_grad_workspace(int64_t n, int64_t hidden);
+
+/* Log-probabilities of given tokens, entropy and the top alternatives of logits / temperature in
+ * one read of the logits (beside tb_head_stats_grad, solution/head.py:34-76). logits [rows, vocab]
+ * in `type`, rows ld elements apart; ids (int64, or int32 when ids_int64 is 0): logprob[r] =
+ * log softmax(logits[r] / temperature)[ids[r]], 0 where ids[r] is outside [0, vocab); entropy[r];
+ * top_logprobs / top_ids [rows, top_k] (top_k 0 to 32): the largest, equal ones by the lowest
+ * index. stats fp32 [rows, 2] is what the backward needs. A row of -inf only gives logprob -inf
+ * and entropy 0; a NaN or +inf makes its row's results NaN (top_ids in range). Temperature 1e-4 to
+ * 1e4, rows below 2^21. `workspace`: tb_token_logprobs_workspace bytes, 16-byte aligned. */
+int tb_token_logprobs_fwd(const void *logits, int32_t type, int64_t ld, const void *ids,
+                          int32_t ids_int64, float temperature, int32_t top_k, float *logprob,
+                          float *entropy, float *top_logprobs, int64_t *top_ids, float *stats,
+                          int64_t rows, int64_t vocab, void *workspace, int64_t workspace_bytes,
+                          void *stream);
+
+/* Its gradient: grad [rows, vocab] in `type`, rows ld_grad apart, for the gradients of logprob,
+ * entropy and top_logprobs (each may be NULL: zero): (1/T) (g_lp (1_id - p) + sum_j g_top_j
+ * (1_top_j - p) - g_H p (log p + H)); zero on rows of -inf only. grad's rows must lie modulo 16
+ * bytes as the logits' rows do (TB_EALIGN otherwise). */
+int tb_token_logprobs_bwd(const void *logits, int32_t type, int64_t ld, const void *ids,
+                          int32_t ids_int64, float temperature, int32_t top_k,
+                          const int64_t *top_ids, const float *stats, const float *entropy,
+                          const float *g_logprob, const float *g_entropy, const float *g_top,
+                          void *grad, int64_t ld_grad, int64_t rows, int64_t vocab, void *stream);
+
+/* Bytes of workspace tb_token_logprobs_fwd needs on the current device (0: none). */
+int64_t tb_token_logprobs_workspace(int64_t rows, int64_t vocab, int32_t type, int32_t top_k);
 
 #ifdef __cplusplus
 }

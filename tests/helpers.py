@@ -105,3 +105,25 @@ def nf4_weight(q, device):
                             code=torch.from_numpy(q["table"]).to(device), dtype=torch.float16)
     data = torch.from_numpy(np.ascontiguousarray(q["packed"]).reshape(-1, 1)).to(device)
     return SimpleNamespace(data=data, quant_state=state)
+
+
+def assert_rounded(got, exact, extra=0.0, what=""):
+    """`got` (a fp16 / bf16 / fp32 tensor) is `exact` (fp64) computed with an absolute error of at
+    most `extra` and rounded once: half a step of its type relative to the value (and half the
+    smallest subnormal) on top of `extra`. NaN and infinities must agree."""
+    g = got.detach().cpu().double()
+    e = torch.as_tensor(exact).double().reshape(g.shape)
+    extra = torch.as_tensor(extra).double()
+    extra = extra.reshape(g.shape) if extra.numel() == g.numel() else extra.expand(g.shape)
+    assert torch.equal(torch.isnan(g), torch.isnan(e)), f"{what}: NaN positions differ"
+    inf = torch.isinf(e) | torch.isnan(e)
+    assert torch.equal(g[torch.isinf(e)], e[torch.isinf(e)]), f"{what}: infinities differ"
+    info = torch.finfo(got.dtype)
+    lim = (e.abs() + extra) * (info.eps / 2) + extra + info.tiny * info.eps / 2
+    err = torch.where(inf, torch.zeros_like(e), (g - e).abs())
+    lim = torch.where(inf, torch.ones_like(e), lim)
+    bad = err > lim
+    if bad.any():
+        i = int((err / lim).argmax())
+        raise AssertionError(f"{what}: {int(bad.sum())} of {bad.numel()} off; worst at {i}: "
+                             f"{g.flatten()[i]} against {e.flatten()[i]}, limit {lim.flatten()[i]}")

@@ -79,13 +79,34 @@ SIGNATURES = {
     "tb_head_dh": [_P, _I64, _P, _P, _I64, _I64, _I64, _F, _P, _I64, _P, _I64, _P, _I32, _P,
                    _I64, _I32, _P],
     "tb_head_dh_workspace": [_I64, _I64, _I64],
+    "tb_dropout": [_P, _I32, _P, _P, _I32, _I64, _I64, _F, _I64, _I64, _P, _P, _P],
+    "tb_norm_rope_fwd": [_P, _I32, _I64, _P, _P, _I32, _P, _P, _I32, _F, _F, _P, _P, _I32, _P, _P,
+                         _P, _P, _I64, _I64, _I64, _I32, _I32, _I32, _P],
+    "tb_norm_rope_bwd": [_P, _P, _P, _P, _I32, _I64, _P, _I32, _P, _P, _I32, _F, _F, _P, _P, _I32,
+                         _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I32, _I32, _I32, _P],
+    "tb_norm_rope_bwd_workspace": [_I64, _I32],
+    "tb_embedding_fwd": [_P, _I32, _P, _I32, _I64, _P, _I32, _F, _I64, _I64, _I64, _P],
+    "tb_embedding_grad": [_P, _I32, _P, _I32, _P, _I32, _F, _I64, _I32, _I64, _I64, _I64, _P, _I64,
+                          _P],
+    "tb_embedding_grad_workspace": [_I64, _I64],
+    "tb_token_logprobs_fwd": [_P, _I32, _I64, _P, _I32, _F, _I32, _P, _P, _P, _P, _P, _I64, _I64,
+                              _P, _I64, _P],
+    "tb_token_logprobs_bwd": [_P, _I32, _I64, _P, _I32, _F, _I32, _P, _P, _P, _P, _P, _P, _P, _I64,
+                              _I64, _I64, _P],
+    "tb_token_logprobs_workspace": [_I64, _I64, _I32, _I32],
 }
 
 # return types other than int (0 or a negative TB_E* code)
 RESTYPES = {"tb_nf4_gemm_workspace": ctypes.c_int64,
             "tb_nf4_gemm_qkv_rope_workspace": ctypes.c_int64,
             "tb_head_dh_workspace": ctypes.c_int64, "tb_launch_count": ctypes.c_int64,
-            "tb_embed_invalid_ids": ctypes.c_int64}
+            "tb_embed_invalid_ids": ctypes.c_int64,
+            "tb_norm_rope_bwd_workspace": ctypes.c_int64,
+            "tb_embedding_grad_workspace": ctypes.c_int64,
+            "tb_token_logprobs_workspace": ctypes.c_int64}
+
+# element types as the C ABI names them (TB_FP16 / TB_BF16 / TB_FP32)
+TYPE_CODES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
 _lib = None
 _calls = 0
@@ -125,6 +146,15 @@ def call(name, *args):
     if rc != 0:
         msg = load().tb_last_error().decode(errors="replace")
         raise KernelError(f"{name} failed ({rc}): {msg}")
+
+
+def call_on(t, name, *args):
+    """call() with the tensor's device current (a kernel launches on the current device, whatever
+    device its stream belongs to)."""
+    if t.device.index == torch.cuda.current_device():
+        return call(name, *args)
+    with torch.cuda.device(t.device):
+        return call(name, *args)
 
 
 def launch_count():

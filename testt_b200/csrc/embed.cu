@@ -9,6 +9,9 @@
 #include "common.cuh"
 
 namespace tb {
+
+unsigned int embedding_invalid_ids(bool &ok);  // embed_grad.cu
+
 namespace {
 
 __device__ unsigned int g_embed_invalid = 0;
@@ -67,5 +70,11 @@ extern "C" int64_t tb_embed_invalid_ids(void) {
     (void)cudaGetLastError();
     return -1;
   }
-  return (int64_t)v;
+  bool ok = false;
+  const unsigned int w = embedding_invalid_ids(ok);
+  if (!ok) {
+    (void)cudaGetLastError();
+    return -1;
+  }
+  return (int64_t)v + (int64_t)w;
 }

@@ -1,0 +1,597 @@
+// Log-probabilities of given tokens with entropy and the top alternatives, from given logits, in
+// one read of them, and their gradient in one read and one write; for sm_100a.
+//   z = logits / T    lse = log sum e^z    p = e^(z - lse)
+//   lp = z[id] - lse    H = lse - sum p z    top: the k largest (value descending, index ascending)
+//   d logits = (1/T) (g_lp (1_id - p) + sum_j g_j (1_top_j - p) - g_H p (log p + H))
+//
+// Forward: an online softmax per thread over the raw logits x: a running maximum m, t = x - m,
+// S = sum 2^(t c) with c = log2(e) / T, U = sum 2^(t c) t; lp = ln2 (t_id c - log2 S) and
+// H = ln2 log2 S - U / (S T). Differences, not products, are taken first, so logits of any size
+// keep their precision. Logits count as kLow = -1e20 at least inside the sums, so a -inf mask (or
+// the type's lowest value) adds 2^.. = 0 and 0 * t stays 0; max.NaN keeps a NaN, which makes the
+// row's results NaN. A row of -inf only has lp -inf, entropy 0 and no gradient.
+//
+// Top k without work per logit: every thread knows its own maximum and where it first was (the
+// softmax needs the maximum anyway). As keys (ordered value << 32 | ~index) all logits differ, and
+// the k-th largest of the threads' maxima is a lower bound of the k-th largest key of the row; only
+// the k threads whose maxima reach it can own logits above it, so only their vectors are read again
+// (from L2). Keys settle ties by the lowest index.
+//
+// Beside the head's statistics over given logits (solution/head.py:34-76, tb_head_stats_grad).
+#include <math_constants.h>
+
+#include "dtypes.cuh"
+
+namespace tb {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kUnroll = 4;       // 16-byte vectors in flight per thread
+constexpr int kMaxTop = 32;      // one list entry per lane
+constexpr float kLow = -1e20f;   // logits below it count as it
+constexpr float kLn2 = 0.693147180559945309f;
+constexpr float kLog2e = 1.44269504088896341f;
+constexpr uint32_t kAll = 0xffffffffu;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
+template <int T>
+constexpr int per_vec() {
+  return 16 / elem_size<T>();
+}
+
+// A row as `head` columns up to a 16-byte boundary, nw whole vectors of E columns and `tail`
+// columns. The (at most 2 E - 2) edge columns go one to a thread of the row's first split.
+struct Row {
+  const char *base;  // column 0
+  int64_t nw;
+  int head, edges;
+};
+
+template <int T>
+__device__ __forceinline__ Row row_of(const void *logits, int64_t row, int64_t ld, int64_t vocab) {
+  constexpr int E = per_vec<T>();
+  Row r;
+  r.base = static_cast<const char *>(logits) + row * ld * elem_size<T>();
+  const int shift = (int)((reinterpret_cast<uintptr_t>(r.base) & 15) / elem_size<T>());
+  r.head = (E - shift) % E;
+  if (r.head > vocab) r.head = (int)vocab;
+  r.nw = (vocab - r.head) / E;
+  r.edges = (int)(vocab - r.nw * E);
+  return r;
+}
+
+// Column of edge j.
+template <int T>
+__device__ __forceinline__ int64_t edge_col(const Row &r, int j) {
+  return j < r.head ? j : r.nw * per_vec<T>() + j;
+}
+
+template <int T>
+__device__ __forceinline__ void unpack_vec(const uint4 &v, float (&z)[per_vec<T>()]) {
+  if constexpr (T == TB_FP32) {
+    z[0] = __uint_as_float(v.x);
+    z[1] = __uint_as_float(v.y);
+    z[2] = __uint_as_float(v.z);
+    z[3] = __uint_as_float(v.w);
+  } else {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = Elem<T>::get2(w[i]);
+      z[2 * i] = f.x;
+      z[2 * i + 1] = f.y;
+    }
+  }
+}
+
+// Whole vector v of the row (columns head + v E + e).
+template <int T>
+__device__ __forceinline__ void load_vec(const Row &r, int64_t v, float (&z)[per_vec<T>()]) {
+  const char *p = r.base + (int64_t)r.head * elem_size<T>() + v * 16;
+  unpack_vec<T>(__ldg(reinterpret_cast<const uint4 *>(p)), z);
+}
+
+// Monotone in (value, then lower index first); -0 counts as +0. 0: nothing.
+__device__ __forceinline__ uint64_t make_key(float z, int64_t c) {
+  const uint32_t b = __float_as_uint(z + 0.f);
+  const uint32_t o = b & 0x80000000u ? ~b : b | 0x80000000u;
+  return (uint64_t)o << 32 | (uint32_t)~(uint32_t)c;
+}
+
+__device__ __forceinline__ float key_value(uint64_t key) {
+  const uint32_t o = (uint32_t)(key >> 32);
+  return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
+}
+
+__device__ __forceinline__ uint32_t key_index(uint64_t key) { return ~(uint32_t)key; }
+
+// The warp's 32 keys in descending order over the lanes.
+__device__ __forceinline__ uint64_t warp_sort(uint64_t key, int lane) {
+#pragma unroll
+  for (int size = 2; size <= 32; size *= 2) {
+#pragma unroll
+    for (int stride = size / 2; stride > 0; stride /= 2) {
+      const uint64_t other = __shfl_xor_sync(kAll, key, stride);
+      const bool lower = (lane & stride) == 0, down = (lane & size) == 0 || size == 32;
+      key = (lower == down) == (key > other) ? key : other;
+    }
+  }
+  return key;
+}
+
+// The 32 largest of two descending lists, descending.
+__device__ __forceinline__ uint64_t warp_merge(uint64_t a, uint64_t b, int lane) {
+  const uint64_t r = __shfl_sync(kAll, b, 31 - lane);
+  uint64_t key = a > r ? a : r;  // bitonic
+#pragma unroll
+  for (int stride = 16; stride > 0; stride /= 2) {
+    const uint64_t other = __shfl_xor_sync(kAll, key, stride);
+    key = ((lane & stride) == 0) == (key > other) ? key : other;
+  }
+  return key;
+}
+
+// Adds each lane's key (0: none) to the warp's descending list when it beats the k-th entry.
+__device__ __forceinline__ void warp_insert(uint64_t &list, uint64_t key, int k, int lane) {
+  const uint64_t kth = __shfl_sync(kAll, list, k - 1);
+  uint32_t todo = __ballot_sync(kAll, key > kth);
+  while (todo) {
+    const int src = __ffs(todo) - 1;
+    todo &= todo - 1;
+    const uint64_t x = __shfl_sync(kAll, key, src);
+    const int place = __popc(__ballot_sync(kAll, list > x));
+    const uint64_t up = __shfl_up_sync(kAll, list, 1);
+    list = lane < place ? list : lane == place ? x : up;
+  }
+}
+
+struct State {  // max, and S and U about max(max, kLow)
+  float m, s, u;
+};
+
+__device__ __forceinline__ float reference(float m) { return fmaxf(m, kLow); }
+
+// (s, u) about m moved to a reference m2 >= m.
+__device__ __forceinline__ void move_to(float &s, float &u, float m, float m2, float c) {
+  const float f = ex2((m - m2) * c);
+  u = f > 0.f ? f * (u + s * (m - m2)) : 0.f;
+  s *= f;
+}
+
+__device__ __forceinline__ State warp_merge_states(State a, float c) {
+  float m = a.m;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kAll, m, o));
+  move_to(a.s, a.u, reference(a.m), reference(m), c);
+  a.m = m;
+  a.s = warp_sum(a.s);
+  a.u = warp_sum(a.u);
+  return a;
+}
+
+struct FwdArgs {
+  const void *logits;
+  const void *ids;  // int64 or int32
+  float *logprob, *entropy, *top_lp, *stats;
+  int64_t *top_ids;
+  float4 *states;       // [rows, splits] partial states (splits > 1)
+  uint64_t *lists;      // [rows, splits, k]
+  int64_t rows, vocab, ld;
+  int64_t split_vecs;   // vectors of a split
+  int splits, k;
+  bool ids64;
+  float c, inv_t;
+};
+
+__device__ __forceinline__ int64_t id_of(const void *ids, bool ids64, int64_t row) {
+  return ids64 ? static_cast<const int64_t *>(ids)[row]
+               : (int64_t)static_cast<const int32_t *>(ids)[row];
+}
+
+// Log-probability of logit x in a row of state a, l = log2 S.
+__device__ __forceinline__ float logprob_of(float x, const State &a, float l, float c,
+                                            float inv_t) {
+  if (x < kLow) return a.m == -CUDART_INF_F ? x : (x - a.m) * inv_t - kLn2 * l;
+  return kLn2 * fmaf(x - reference(a.m), c, -l);
+}
+
+// One warp writes a row's results. key: the row's list over the lanes.
+template <int T>
+__device__ __forceinline__ void finish_row(const FwdArgs &a, int64_t row, const State &st,
+                                           uint64_t key, int lane) {
+  const float l = log2f(st.s);
+  const bool empty = st.m == -CUDART_INF_F && st.s == st.s;
+  if (lane == 0) {
+    const int64_t id = id_of(a.ids, a.ids64, row);
+    float lp = 0.f;
+    if (id >= 0 && id < a.vocab)
+      lp = logprob_of(load1<T>(a.logits, row * a.ld + id), st, l, a.c, a.inv_t);
+    a.logprob[row] = lp;
+    const float h = kLn2 * l - st.u / st.s * a.inv_t;
+    a.entropy[row] = empty || h < 0.f ? 0.f : h;
+    a.stats[2 * row] = reference(st.m);
+    a.stats[2 * row + 1] = empty ? CUDART_INF_F : l;
+  }
+  if (lane < a.k) {
+    a.top_ids[row * a.k + lane] = key == 0 ? 0 : (int64_t)key_index(key);
+    a.top_lp[row * a.k + lane] =
+        key == 0 ? CUDART_NAN_F : logprob_of(key_value(key), st, l, a.c, a.inv_t);
+  }
+}
+
+__device__ __forceinline__ void add_logit(float x, float ref, float c, float &s, float &u) {
+  const float t = max_nan(x, kLow) - ref;
+  const float p = ex2(t * c);
+  s += p;
+  u = fmaf(p, t, u);
+}
+
+template <int T>
+__global__ void __launch_bounds__(kThreads) logprobs_fwd(FwdArgs a) {
+  pdl_wait();
+  pdl_release();
+  constexpr int E = per_vec<T>();
+  __shared__ State sh_state[kWarps];
+  __shared__ uint64_t sh_list[kWarps][32];
+  __shared__ uint64_t sh_bar;
+  __shared__ int sh_n;
+  __shared__ uint16_t sh_who[kThreads];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = blockIdx.x / a.splits;
+  const int split = (int)(blockIdx.x - row * a.splits);
+  const Row r = row_of<T>(a.logits, row, a.ld, a.vocab);
+  const int64_t v0 = split * a.split_vecs;
+  const int64_t v1 = v0 + a.split_vecs < r.nw ? v0 + a.split_vecs : r.nw;
+  const int edges = split == 0 ? r.edges : 0;
+  State st{-CUDART_INF_F, 0.f, 0.f};
+  float ref = reference(st.m);
+  int64_t best = v0 + threadIdx.x;  // first vector of the batch the maximum came from
+  for (int64_t v = v0 + threadIdx.x; v < v1; v += (int64_t)kThreads * kUnroll) {
+    float z[kUnroll][E];
+#pragma unroll
+    for (int b = 0; b < kUnroll; ++b) {
+      const int64_t vb = v + (int64_t)b * kThreads;
+      if (vb < v1) {
+        load_vec<T>(r, vb, z[b]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) z[b][e] = -CUDART_INF_F;
+      }
+    }
+    float m = -CUDART_INF_F;
+#pragma unroll
+    for (int b = 0; b < kUnroll; ++b)
+#pragma unroll
+      for (int e = 0; e < E; ++e) m = fmaxf(m, z[b][e]);
+    if (m > st.m) {
+      move_to(st.s, st.u, ref, reference(m), a.c);
+      ref = reference(m);
+      st.m = m;
+      best = v;
+    }
+#pragma unroll
+    for (int b = 0; b < kUnroll; ++b) {
+      if (v + (int64_t)b * kThreads >= v1) break;
+#pragma unroll
+      for (int e = 0; e < E; ++e) add_logit(z[b][e], ref, a.c, st.s, st.u);
+    }
+  }
+  const float own_max = st.m;  // of the whole vectors
+  uint64_t edge_key = 0;
+  if ((int)threadIdx.x < edges) {
+    const int64_t col = edge_col<T>(r, threadIdx.x);
+    const float x = load1<T>(r.base, col);
+    if (x == x) edge_key = make_key(x, col);
+    if (x > st.m) {
+      move_to(st.s, st.u, ref, reference(x), a.c);
+      ref = reference(x);
+      st.m = x;
+    }
+    add_logit(x, ref, a.c, st.s, st.u);
+  }
+  State w = warp_merge_states(st, a.c);
+  if (lane == 0) sh_state[warp] = w;
+  uint64_t list = 0;
+  if (a.k > 0) {
+    // this thread's largest key among its whole vectors: its maximum's first place
+    uint64_t mine = 0;
+    for (int b = 0; b < kUnroll && mine == 0; ++b) {
+      const int64_t vb = best + (int64_t)b * kThreads;
+      if (vb >= v1) break;
+      float z[E];
+      load_vec<T>(r, vb, z);
+#pragma unroll
+      for (int e = E - 1; e >= 0; --e)
+        if (z[e] == own_max) mine = make_key(z[e], r.head + vb * E + e);
+    }
+    sh_list[warp][lane] = warp_sort(mine, lane);
+    if (threadIdx.x == 0) sh_n = 0;
+    __syncthreads();
+    if (warp == 0) {
+      uint64_t top = sh_list[0][lane];
+#pragma unroll
+      for (int i = 1; i < kWarps; ++i) top = warp_merge(top, sh_list[i][lane], lane);
+      top = __shfl_sync(kAll, top, a.k - 1);
+      if (lane == 0) sh_bar = top;
+    }
+    __syncthreads();
+    const uint64_t bar = sh_bar;
+    if (mine != 0 && mine >= bar) sh_who[atomicAdd(&sh_n, 1)] = (uint16_t)threadIdx.x;
+    __syncthreads();
+    // the owners' vectors once more, and the edges (the first warp holds them all)
+    if (warp == 0) warp_insert(list, edge_key < bar ? 0 : edge_key, a.k, lane);
+    const int64_t each = (v1 - v0 + kThreads - 1) / kThreads;
+    const int64_t items = each * sh_n;
+    for (int64_t i0 = (int64_t)warp * 32; i0 < items; i0 += kThreads) {
+      const int64_t i = i0 + lane;
+      int64_t vb = v1;
+      if (i < items) vb = v0 + sh_who[i / each] + (i % each) * kThreads;
+      float z[E];
+      if (vb < v1) load_vec<T>(r, vb, z);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        uint64_t key = 0;
+        if (vb < v1 && z[e] == z[e]) key = make_key(z[e], r.head + vb * E + e);
+        warp_insert(list, key < bar ? 0 : key, a.k, lane);
+      }
+    }
+    sh_list[warp][lane] = list;  // the maxima were read before the last barrier but one
+  }
+  __syncthreads();
+  if (warp != 0) return;
+  w = lane < kWarps ? sh_state[lane] : State{-CUDART_INF_F, 0.f, 0.f};
+  w = warp_merge_states(w, a.c);
+  if (a.k > 0) {
+#pragma unroll
+    for (int i = 1; i < kWarps; ++i) list = warp_merge(list, sh_list[i][lane], lane);
+  }
+  if (a.splits == 1) {
+    finish_row<T>(a, row, w, list, lane);
+  } else {
+    if (lane == 0) a.states[blockIdx.x] = make_float4(w.m, w.s, w.u, 0.f);
+    if (lane < a.k) a.lists[(int64_t)blockIdx.x * a.k + lane] = list;
+  }
+}
+
+// A warp per row over its splits' states and lists.
+template <int T>
+__global__ void __launch_bounds__(32) logprobs_merge(FwdArgs a) {
+  pdl_wait();
+  pdl_release();
+  const int lane = threadIdx.x;
+  const int64_t row = blockIdx.x;
+  State w{-CUDART_INF_F, 0.f, 0.f};
+  for (int i = lane; i < a.splits; i += 32) {
+    const float4 q = a.states[row * a.splits + i];
+    State o{q.x, q.y, q.z};
+    const float m = fmaxf(w.m, o.m);
+    move_to(w.s, w.u, reference(w.m), reference(m), a.c);
+    move_to(o.s, o.u, reference(o.m), reference(m), a.c);
+    w = State{m, w.s + o.s, w.u + o.u};
+  }
+  w = warp_merge_states(w, a.c);
+  uint64_t list = 0;
+  const int64_t keys = (int64_t)a.splits * a.k;
+  for (int64_t i0 = 0; i0 < keys; i0 += 32) {
+    const int64_t i = i0 + lane;
+    warp_insert(list, i < keys ? a.lists[row * keys + i] : 0, a.k, lane);
+  }
+  finish_row<T>(a, row, w, list, lane);
+}
+
+struct BwdArgs {
+  const void *logits;
+  const void *ids;
+  const int64_t *top_ids;
+  const float *stats, *entropy, *g_lp, *g_ent, *g_top;
+  void *grad;
+  int64_t rows, vocab, ld, ld_grad, split_vecs;
+  int splits, k;
+  bool ids64;
+  float c, inv_t;
+};
+
+// p (G + g_H (log p + H)) of a logit: d = log2 p, A and B hold the factors.
+__device__ __forceinline__ float slope(float x, float ref, float l, float c, float A, float B) {
+  const float d = fmaf(max_nan(x, kLow) - ref, c, -l);
+  return ex2(d) * fmaf(B, d, A);
+}
+
+template <int T>
+__global__ void __launch_bounds__(kThreads) logprobs_bwd(BwdArgs a) {
+  pdl_wait();
+  pdl_release();
+  constexpr int E = per_vec<T>();
+  __shared__ int64_t sh_col[kMaxTop + 1];
+  __shared__ float sh_g[kMaxTop + 1];
+  const int64_t row = blockIdx.x / a.splits;
+  const int split = (int)(blockIdx.x - row * a.splits);
+  const Row r = row_of<T>(a.logits, row, a.ld, a.vocab);
+  char *out = static_cast<char *>(a.grad) + row * a.ld_grad * elem_size<T>();
+  char *out_vecs = out + (int64_t)r.head * elem_size<T>();
+  const int64_t v0 = split * a.split_vecs;
+  const int64_t v1 = v0 + a.split_vecs < r.nw ? v0 + a.split_vecs : r.nw;
+  const int edges = split == 0 ? r.edges : 0;
+  if ((int)threadIdx.x <= a.k) {
+    const int j = threadIdx.x;
+    int64_t col = j == 0 ? id_of(a.ids, a.ids64, row) : a.top_ids[row * a.k + j - 1];
+    float g = j == 0 ? (a.g_lp ? a.g_lp[row] : 0.f) : (a.g_top ? a.g_top[row * a.k + j - 1] : 0.f);
+    if (col < 0 || col >= a.vocab) {
+      col = -1;
+      g = 0.f;
+    }
+    sh_col[j] = col;
+    sh_g[j] = g;
+  }
+  __syncthreads();
+  float G = 0.f;
+  for (int j = 0; j <= a.k; ++j) G += sh_g[j];
+  const float ref = a.stats[2 * row];
+  const bool empty = a.stats[2 * row + 1] == CUDART_INF_F;
+  const float l = empty ? 0.f : a.stats[2 * row + 1];
+  const float gh = a.g_ent ? a.g_ent[row] : 0.f;
+  const float A = empty ? 0.f : -a.inv_t * (G + gh * a.entropy[row]);
+  const float B = empty ? 0.f : -a.inv_t * gh * kLn2;
+  for (int64_t v = v0 + threadIdx.x; v < v1; v += (int64_t)kThreads * kUnroll) {
+    float z[kUnroll][E];
+#pragma unroll
+    for (int b = 0; b < kUnroll; ++b) {
+      const int64_t vb = v + (int64_t)b * kThreads;
+      if (vb < v1) load_vec<T>(r, vb, z[b]);
+    }
+#pragma unroll
+    for (int b = 0; b < kUnroll; ++b) {
+      const int64_t vb = v + (int64_t)b * kThreads;
+      if (vb >= v1) break;
+#pragma unroll
+      for (int e = 0; e < E; ++e) z[b][e] = slope(z[b][e], ref, l, a.c, A, B);
+      uint4 w;
+      if constexpr (T == TB_FP32)
+        w = make_uint4(__float_as_uint(z[b][0]), __float_as_uint(z[b][1]),
+                       __float_as_uint(z[b][2]), __float_as_uint(z[b][3]));
+      else
+        w = make_uint4(Elem<T>::put2(z[b][0], z[b][1]), Elem<T>::put2(z[b][2], z[b][3]),
+                       Elem<T>::put2(z[b][4 % E], z[b][5 % E]),
+                       Elem<T>::put2(z[b][6 % E], z[b][7 % E]));
+      *reinterpret_cast<uint4 *>(out_vecs + vb * 16) = w;
+    }
+  }
+  if ((int)threadIdx.x < edges) {
+    const int64_t col = edge_col<T>(r, threadIdx.x);
+    store1<T>(out, col, slope(load1<T>(r.base, col), ref, l, a.c, A, B));
+  }
+  if (empty) return;
+  __syncthreads();  // the given and top columns are written again, with their one-hot terms
+  if ((int)threadIdx.x <= a.k && sh_col[threadIdx.x] >= 0) {
+    const int64_t col = sh_col[threadIdx.x], v = (col - r.head) / E;
+    const bool edge = col < r.head || v >= r.nw;
+    if (edge ? split == 0 : v >= v0 && v < v1) {
+      float g = 0.f;
+      for (int j = 0; j <= a.k; ++j) g += sh_col[j] == col ? sh_g[j] : 0.f;
+      store1<T>(out, col, fmaf(g, a.inv_t, slope(load1<T>(r.base, col), ref, l, a.c, A, B)));
+    }
+  }
+}
+
+// Splits of a row: enough CTAs for the device when there are few rows.
+int64_t splits_of(int64_t rows, int64_t vecs, int64_t target) {
+  int64_t s = (target + rows - 1) / rows;
+  const int64_t most = (vecs + kThreads - 1) / kThreads;
+  if (s > most) s = most;
+  return s < 1 ? 1 : s;
+}
+
+int64_t most_vecs(int64_t vocab, int es) { return (vocab * es + 15) / 16; }
+
+int check(const char *what, int64_t rows, int64_t vocab, int64_t ld, int type, int k, float t) {
+  if (rows < 0 || vocab <= 0 || vocab > 0x7fffffffLL || rows > 0x7fffffffLL / 1024 ||
+      (rows > 1 && ld < vocab))
+    return set_error(TB_EINVAL, "%s: rows %lld vocab %lld row stride %lld", what, (long long)rows,
+                     (long long)vocab, (long long)ld);
+  if (!elem_type_ok(type)) return set_error(TB_EINVAL, "%s: type %d", what, type);
+  if (k < 0 || k > kMaxTop || k > vocab)
+    return set_error(TB_EINVAL, "%s: top %d (0 to %d, at most the vocabulary)", what, k, kMaxTop);
+  if (!(t >= 1e-4f && t <= 1e4f))
+    return set_error(TB_EINVAL, "%s: temperature %g outside [1e-4, 1e4]", what, (double)t);
+  return TB_OK;
+}
+
+int64_t fwd_splits(int64_t rows, int64_t vocab, int type) {
+  return splits_of(rows, most_vecs(vocab, elem_size_of(type)), (int64_t)sm_count() * 4);
+}
+
+}  // namespace
+}  // namespace tb
+
+using namespace tb;
+
+extern "C" int64_t tb_token_logprobs_workspace(int64_t rows, int64_t vocab, int32_t type,
+                                               int32_t top_k) {
+  if (rows <= 0 || vocab <= 0 || top_k < 0 || !elem_type_ok(type)) return 0;
+  const int64_t s = fwd_splits(rows, vocab, type);
+  return s > 1 ? rows * s * (16 + 8 * (int64_t)top_k) : 0;
+}
+
+extern "C" int tb_token_logprobs_fwd(const void *logits, int32_t type, int64_t ld, const void *ids,
+                                     int32_t ids_int64, float temperature, int32_t top_k,
+                                     float *logprob, float *entropy, float *top_logprobs,
+                                     int64_t *top_ids, float *stats, int64_t rows, int64_t vocab,
+                                     void *workspace, int64_t workspace_bytes, void *stream) {
+  int rc = check("token_logprobs_fwd", rows, vocab, ld, type, top_k, temperature);
+  if (rc != TB_OK) return rc;
+  if (rows == 0) return TB_OK;
+  if (!logits || !ids || !logprob || !entropy || !stats || (top_k > 0 && (!top_logprobs || !top_ids)))
+    return set_error(TB_EINVAL, "token_logprobs_fwd: a buffer is missing");
+  if (!aligned(logits, elem_size_of(type)) || !aligned(ids, ids_int64 ? 8 : 4) ||
+      !aligned(logprob, 4) || !aligned(entropy, 4) || !aligned(stats, 4) ||
+      !aligned(top_logprobs, 4) || !aligned(top_ids, 8) || !aligned(workspace, 16))
+    return set_error(TB_EALIGN, "token_logprobs_fwd: a buffer is not aligned to its element");
+  const int64_t need = tb_token_logprobs_workspace(rows, vocab, type, top_k);
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return set_error(TB_EINVAL, "token_logprobs_fwd: workspace of %lld bytes, %lld needed",
+                     (long long)workspace_bytes, (long long)need);
+  const int64_t splits = fwd_splits(rows, vocab, type);
+  const int64_t nv = most_vecs(vocab, elem_size_of(type));
+  char *ws = static_cast<char *>(workspace);
+  const FwdArgs a{logits, ids, logprob, entropy, top_logprobs, stats, top_ids,
+                  reinterpret_cast<float4 *>(ws),
+                  reinterpret_cast<uint64_t *>(ws + rows * splits * 16), rows, vocab, ld,
+                  (nv + splits - 1) / splits, (int)splits, top_k, ids_int64 != 0,
+                  kLog2e / temperature, 1.f / temperature};
+  cudaStream_t st = as_stream(stream);
+  TB_WITH_TYPE(type, T,
+               rc = launch("token_logprobs_fwd", logprobs_fwd<T>, dim3((unsigned)(rows * splits)),
+                           kThreads, 0, st, a);
+               if (rc == TB_OK && splits > 1) rc =
+                   launch("token_logprobs_fwd", logprobs_merge<T>, dim3((unsigned)rows), 32, 0, st,
+                          a));
+  return rc;
+}
+
+extern "C" int tb_token_logprobs_bwd(const void *logits, int32_t type, int64_t ld, const void *ids,
+                                     int32_t ids_int64, float temperature, int32_t top_k,
+                                     const int64_t *top_ids, const float *stats,
+                                     const float *entropy, const float *g_logprob,
+                                     const float *g_entropy, const float *g_top, void *grad,
+                                     int64_t ld_grad, int64_t rows, int64_t vocab, void *stream) {
+  int rc = check("token_logprobs_bwd", rows, vocab, ld, type, top_k, temperature);
+  if (rc != TB_OK) return rc;
+  if (rows == 0) return TB_OK;
+  if (!logits || !ids || !stats || !entropy || !grad || (top_k > 0 && !top_ids))
+    return set_error(TB_EINVAL, "token_logprobs_bwd: a buffer is missing");
+  if (rows > 1 && ld_grad < vocab)
+    return set_error(TB_EINVAL, "token_logprobs_bwd: gradient row stride %lld", (long long)ld_grad);
+  const int es = elem_size_of(type);
+  if (!aligned(logits, es) || !aligned(ids, ids_int64 ? 8 : 4) || !aligned(top_ids, 8) ||
+      !aligned(stats, 4) || !aligned(entropy, 4) || !aligned(g_logprob, 4) ||
+      !aligned(g_entropy, 4) || !aligned(g_top, 4))
+    return set_error(TB_EALIGN, "token_logprobs_bwd: a buffer is not aligned to its element");
+  // each gradient row lies in its 16-byte words as the logits' row does
+  if (((reinterpret_cast<uintptr_t>(logits) ^ reinterpret_cast<uintptr_t>(grad)) & 15) != 0 ||
+      (rows > 1 && (ld - ld_grad) * es % 16 != 0))
+    return set_error(TB_EALIGN, "token_logprobs_bwd: the gradient's rows must lie modulo 16 bytes "
+                                "as the logits' rows do");
+  const int64_t nv = most_vecs(vocab, es);
+  const int64_t per = (int64_t)kThreads * kUnroll * 2;
+  int64_t splits = (nv + per - 1) / per;
+  if (splits > 1024) splits = 1024;
+  const BwdArgs a{logits, ids, top_ids, stats, entropy, g_logprob, g_entropy, g_top, grad, rows,
+                  vocab, ld, ld_grad, (nv + splits - 1) / splits, (int)splits, top_k,
+                  ids_int64 != 0, kLog2e / temperature, 1.f / temperature};
+  cudaStream_t st = as_stream(stream);
+  TB_WITH_TYPE(type, T,
+               return launch("token_logprobs_bwd", logprobs_bwd<T>,
+                             dim3((unsigned)(rows * splits)), kThreads, 0, st, a));
+}

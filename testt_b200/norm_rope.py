@@ -1,0 +1,135 @@
+"""Per-head RMS norms of queries and keys, the LoRA add and the rotary embedding in one pass on
+B200 (tb_norm_rope_fwd / tb_norm_rope_bwd): rope.rope_tokens (reference: solution/rope.py) for
+decoders that norm each query and key head before the rotation.
+
+    x = qkv + lora                                            fp32
+    q, k: n = x * rsqrt(mean(x^2 over the head) + eps) * (weight_offset + weight)
+          y = n cos + half-turned n sin on the first rot dims, n past them
+    v = x
+Outputs are token-major (q [rows, n_heads, d], k and v [rows, n_kv, d]), the layout
+attention.varlen_attention takes. The forward keeps nothing but its inputs: the backward forms
+the norms again from them.
+"""
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+
+
+def _ld(qkv):
+    """Elements between rows (a single row's stride may be anything)."""
+    return qkv.stride(0) if qkv.shape[0] > 1 else qkv.shape[1]
+
+
+def _code(t, default):
+    return default if t is None else _lib.TYPE_CODES[t.dtype]
+
+
+class NormRopeTokens(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, qkv, lora_q, lora_v, q_weight, k_weight, eps, cos, sin, pos_idx, batch, seq,
+                n_heads, n_kv, head_dim, weight_offset):
+        rows, dev, dt = qkv.shape[0], qkv.device, qkv.dtype
+        code = _lib.TYPE_CODES[dt]
+        q = torch.empty((rows, n_heads, head_dim), dtype=dt, device=dev)
+        k = torch.empty((rows, n_kv, head_dim), dtype=dt, device=dev)
+        v = torch.empty((rows, n_kv, head_dim), dtype=dt, device=dev)
+        if rows:
+            _lib.call_on(qkv, "tb_norm_rope_fwd", _lib.ptr(qkv), code, _ld(qkv),
+                         _lib.ptr(lora_q), _lib.ptr(lora_v),
+                         _code(lora_q if lora_q is not None else lora_v, code),
+                         _lib.ptr(q_weight), _lib.ptr(k_weight),
+                         _code(q_weight if q_weight is not None else k_weight, code),
+                         weight_offset, eps, _lib.ptr(cos), _lib.ptr(sin), cos.shape[1],
+                         _lib.ptr(pos_idx), _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), rows, batch,
+                         seq, n_heads, n_kv, head_dim, _lib.stream_of(qkv))
+        ctx.save_for_backward(qkv, lora_q, q_weight, k_weight, cos, sin, pos_idx)
+        ctx.dims = (eps, batch, seq, n_heads, n_kv, head_dim, weight_offset)
+        ctx.set_materialize_grads(False)
+        return q, k, v
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_q, grad_k, grad_v):
+        qkv, lora_q, q_weight, k_weight, cos, sin, pos_idx = ctx.saved_tensors
+        eps, batch, seq, n_heads, n_kv, head_dim, weight_offset = ctx.dims
+        need = ctx.needs_input_grad
+        rows, dev = qkv.shape[0], qkv.device
+        code = _lib.TYPE_CODES[qkv.dtype]
+        grads = [None if g is None else g.contiguous() for g in (grad_q, grad_k, grad_v)]
+        dqkv = torch.empty((rows, (n_heads + 2 * n_kv) * head_dim), dtype=qkv.dtype, device=dev)
+        dqw = torch.empty_like(q_weight) if need[3] else None
+        dkw = torch.empty_like(k_weight) if need[4] else None
+        ws, nbytes = None, 0
+        if dqw is not None or dkw is not None:
+            with torch.cuda.device(dev):
+                nbytes = _lib.load().tb_norm_rope_bwd_workspace(rows, head_dim)
+            ws = torch.empty(max(nbytes // 4, 1), dtype=torch.float32, device=dev)
+        _lib.call_on(qkv, "tb_norm_rope_bwd", _lib.ptr(grads[0]), _lib.ptr(grads[1]),
+                     _lib.ptr(grads[2]), _lib.ptr(qkv), code, _ld(qkv), _lib.ptr(lora_q),
+                     _code(lora_q, code), _lib.ptr(q_weight), _lib.ptr(k_weight),
+                     _code(q_weight if q_weight is not None else k_weight, code), weight_offset,
+                     eps, _lib.ptr(cos), _lib.ptr(sin), cos.shape[1], _lib.ptr(pos_idx),
+                     _lib.ptr(dqkv), _lib.ptr(dqw), _lib.ptr(dkw), _lib.ptr(ws), nbytes, rows,
+                     batch, seq, n_heads, n_kv, head_dim, _lib.stream_of(qkv))
+        q_cols, v_start = n_heads * head_dim, (n_heads + n_kv) * head_dim
+        return (dqkv if need[0] else None, dqkv[:, :q_cols] if need[1] else None,
+                dqkv[:, v_start:] if need[2] else None, dqw, dkw, None, None, None, None, None,
+                None, None, None, None, None)
+
+
+def _pair(a, b, dtype):
+    """Two optional tensors contiguous and in one type the kernels take (`dtype`'s or fp32)."""
+    if (a is None or a.dtype == dtype) and (b is None or b.dtype == dtype):
+        return None if a is None else a.contiguous(), None if b is None else b.contiguous()
+    return (None if a is None else a.to(torch.float32).contiguous(),
+            None if b is None else b.to(torch.float32).contiguous())
+
+
+def norm_rope_tokens(qkv, lora_q, lora_v, q_weight, k_weight, eps, cos, sin, pos_idx, batch, seq,
+                     n_heads, n_kv, head_dim, weight_offset=0.0):
+    """(q, k, v) token-major in qkv's dtype (fp16, bf16 or fp32), as rope.rope_tokens with each
+    query and key head normed first. `lora_q` [rows, n_heads * head_dim] and `lora_v` [rows,
+    n_kv * head_dim] are added in fp32 (None: none); `q_weight`, `k_weight` [head_dim] (None: 1);
+    `cos`, `sin` [>= seq, rot] with rot <= head_dim; a token's table row is pos_idx % seq, and one
+    whose pos_idx is outside [0, batch * seq) gets zero rows and no gradient. qkv's rows may be
+    views of wider rows. Differentiable in qkv, lora_q, lora_v, q_weight and k_weight."""
+    _lib.require_cuda(qkv, lora_q, lora_v, q_weight, k_weight, cos, sin, pos_idx,
+                      what="norm_rope_tokens")
+    if qkv.dtype not in _lib.TYPE_CODES:
+        raise TypeError(f"norm_rope_tokens: qkv must be fp16, bf16 or fp32, got {qkv.dtype}")
+    if n_heads <= 0 or n_kv < 0 or head_dim <= 0 or head_dim % 2:
+        raise ValueError(f"norm_rope_tokens: {n_heads} / {n_kv} heads of {head_dim}")
+    if qkv.dim() != 2 or qkv.shape[1] != (n_heads + 2 * n_kv) * head_dim:
+        raise ValueError(f"norm_rope_tokens: qkv {tuple(qkv.shape)}, expected "
+                         f"[rows, {(n_heads + 2 * n_kv) * head_dim}]")
+    rows = qkv.shape[0]
+    for name, t, shape in (("lora_q", lora_q, (rows, n_heads * head_dim)),
+                           ("lora_v", lora_v, (rows, n_kv * head_dim)),
+                           ("q_weight", q_weight, (head_dim,)), ("k_weight", k_weight, (head_dim,)),
+                           ("pos_idx", pos_idx, (rows,))):
+        if t is not None and tuple(t.shape) != shape:
+            raise ValueError(f"norm_rope_tokens: {name} {tuple(t.shape)}, expected {shape}")
+    for t in (lora_q, lora_v, q_weight, k_weight):
+        if t is not None and t.dtype not in _lib.TYPE_CODES:
+            raise TypeError(f"norm_rope_tokens: LoRA rows and weights are fp16, bf16 or fp32, "
+                            f"got {t.dtype}")
+    if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[0] < seq or cos.shape[1] % 2 or \
+            cos.shape[1] > head_dim:
+        raise ValueError(f"norm_rope_tokens: tables {tuple(cos.shape)} and {tuple(sin.shape)} for "
+                         f"seq {seq}, head_dim {head_dim}")
+    if pos_idx.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"norm_rope_tokens: pos_idx must be int64 or int32, got {pos_idx.dtype}")
+    for t in (lora_q, lora_v, q_weight, k_weight, cos, sin, pos_idx):
+        if t is not None and t.device != qkv.device:
+            raise ValueError(f"norm_rope_tokens: operands on {t.device} and {qkv.device}")
+    if qkv.stride(1) != 1 or _ld(qkv) < qkv.shape[1]:
+        qkv = qkv.contiguous()
+    lora_q, lora_v = _pair(lora_q, lora_v, qkv.dtype)
+    q_weight, k_weight = _pair(q_weight, k_weight, qkv.dtype)
+    return NormRopeTokens.apply(qkv, lora_q, lora_v, q_weight, k_weight, float(eps),
+                                cos.to(torch.float32).contiguous(),
+                                sin.to(torch.float32).contiguous(),
+                                pos_idx.to(torch.int64).contiguous(), int(batch), int(seq),
+                                int(n_heads), int(n_kv), int(head_dim), float(weight_offset))
