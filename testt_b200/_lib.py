@@ -150,11 +150,37 @@ def call(name, *args):
 
 def call_on(t, name, *args):
     """call() with the tensor's device current (a kernel launches on the current device, whatever
-    device its stream belongs to)."""
-    if t.device.index == torch.cuda.current_device():
-        return call(name, *args)
-    with torch.cuda.device(t.device):
-        return call(name, *args)
+    device its stream belongs to) and the device's current stream as the last argument. Pointers
+    are passed as addr() gives them: a launch from Python costs 6 us less than with ctypes objects
+    and a Stream object (14 against 20 us for a dropout call of 4096 elements)."""
+    index = t.get_device()
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
+            return call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+    return call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+
+
+def workspace_bytes(t, name, *args):
+    """A workspace size (which may depend on the device) with the tensor's device current."""
+    index = t.get_device()
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
+            return getattr(load(), name)(*args)
+    return getattr(load(), name)(*args)
+
+
+def addr(t):
+    """Device address of a tensor as an int (None for None)."""
+    return None if t is None else t.data_ptr()
+
+
+def needs_grad(*tensors):
+    """Whether autograd would record a call on these tensors."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def launch_count():

@@ -11,11 +11,11 @@
 // the type's lowest value) adds 2^.. = 0 and 0 * t stays 0; max.NaN keeps a NaN, which makes the
 // row's results NaN. A row of -inf only has lp -inf, entropy 0 and no gradient.
 //
-// Top k without work per logit: every thread knows its own maximum and where it first was (the
-// softmax needs the maximum anyway). As keys (ordered value << 32 | ~index) all logits differ, and
-// the k-th largest of the threads' maxima is a lower bound of the k-th largest key of the row; only
-// the k threads whose maxima reach it can own logits above it, so only their vectors are read again
-// (from L2). Keys settle ties by the lowest index.
+// Top k without work per logit: every thread knows its own maximum (the softmax needs it anyway).
+// The k-th largest of the threads' maxima is a lower bound of the row's k-th largest logit, and
+// only threads whose maxima reach it (k of them, more with ties) own logits that do, so only their
+// vectors are read again (from L2). Those logits become keys (ordered value << 32 | ~index), which
+// all differ and settle ties by the lowest index, in descending lists over a warp's lanes.
 //
 // Beside the head's statistics over given logits (solution/head.py:34-76, tb_head_stats_grad).
 #include <math_constants.h>
@@ -28,6 +28,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kUnroll = 4;       // 16-byte vectors in flight per thread
+constexpr int kAgain = 2;        // vectors in flight per thread when they are read again
 constexpr int kMaxTop = 32;      // one list entry per lane
 constexpr float kLow = -1e20f;   // logits below it count as it
 constexpr float kLn2 = 0.693147180559945309f;
@@ -103,6 +104,13 @@ __device__ __forceinline__ void load_vec(const Row &r, int64_t v, float (&z)[per
   unpack_vec<T>(__ldg(reinterpret_cast<const uint4 *>(p)), z);
 }
 
+// A batch: the vectors p, p + kThreads, ..., N of them, in flight together.
+template <int N>
+__device__ __forceinline__ void load_batch(const uint4 *p, uint4 (&raw)[N]) {
+#pragma unroll
+  for (int b = 0; b < N; ++b) raw[b] = __ldg(p + b * kThreads);
+}
+
 // Monotone in (value, then lower index first); -0 counts as +0. 0: nothing.
 __device__ __forceinline__ uint64_t make_key(float z, int64_t c) {
   const uint32_t b = __float_as_uint(z + 0.f);
@@ -117,30 +125,48 @@ __device__ __forceinline__ float key_value(uint64_t key) {
 
 __device__ __forceinline__ uint32_t key_index(uint64_t key) { return ~(uint32_t)key; }
 
-// The warp's 32 keys in descending order over the lanes.
-__device__ __forceinline__ uint64_t warp_sort(uint64_t key, int lane) {
+// The warp's 32 values in descending order over the lanes.
+__device__ __forceinline__ float warp_sort(float v, int lane) {
 #pragma unroll
   for (int size = 2; size <= 32; size *= 2) {
 #pragma unroll
     for (int stride = size / 2; stride > 0; stride /= 2) {
-      const uint64_t other = __shfl_xor_sync(kAll, key, stride);
+      const float other = __shfl_xor_sync(kAll, v, stride);
       const bool lower = (lane & stride) == 0, down = (lane & size) == 0 || size == 32;
-      key = (lower == down) == (key > other) ? key : other;
+      v = lower == down ? fmaxf(v, other) : fminf(v, other);
     }
+  }
+  return v;
+}
+
+// The 32 largest of two descending lists, descending.
+template <typename K>
+__device__ __forceinline__ K warp_merge(K a, K b, int lane) {
+  const K r = __shfl_sync(kAll, b, 31 - lane);
+  K key = a > r ? a : r;  // bitonic
+#pragma unroll
+  for (int stride = 16; stride > 0; stride /= 2) {
+    const K other = __shfl_xor_sync(kAll, key, stride);
+    key = ((lane & stride) == 0) == (key > other) ? key : other;
   }
   return key;
 }
 
-// The 32 largest of two descending lists, descending.
-__device__ __forceinline__ uint64_t warp_merge(uint64_t a, uint64_t b, int lane) {
-  const uint64_t r = __shfl_sync(kAll, b, 31 - lane);
-  uint64_t key = a > r ? a : r;  // bitonic
+// The 32 largest of the warps' descending lists in warp 0, by pairs; `sh` [kWarps][32]. Ends with
+// every warp's reads of sh done and warp 0's result its own (and in sh[0]).
+template <typename K>
+__device__ __forceinline__ K block_merge(K list, K (*sh)[32], int warp, int lane) {
+  sh[warp][lane] = list;
+  __syncthreads();
 #pragma unroll
-  for (int stride = 16; stride > 0; stride /= 2) {
-    const uint64_t other = __shfl_xor_sync(kAll, key, stride);
-    key = ((lane & stride) == 0) == (key > other) ? key : other;
+  for (int step = 1; step < kWarps; step *= 2) {
+    if (warp % (2 * step) == 0) {
+      list = warp_merge(list, sh[warp + step][lane], lane);
+      sh[warp][lane] = list;
+    }
+    __syncthreads();
   }
-  return key;
+  return list;
 }
 
 // Adds each lane's key (0: none) to the warp's descending list when it beats the k-th entry.
@@ -165,8 +191,8 @@ __device__ __forceinline__ float reference(float m) { return fmaxf(m, kLow); }
 
 // (s, u) about m moved to a reference m2 >= m.
 __device__ __forceinline__ void move_to(float &s, float &u, float m, float m2, float c) {
-  const float f = ex2((m - m2) * c);
-  u = f > 0.f ? f * (u + s * (m - m2)) : 0.f;
+  const float d = (m - m2) * c, f = ex2(d);
+  u = f > 0.f ? f * (u + s * d) : 0.f;
   s *= f;
 }
 
@@ -180,6 +206,48 @@ __device__ __forceinline__ State warp_merge_states(State a, float c) {
   a.u = warp_sum(a.u);
   return a;
 }
+
+// A thread's running sums. d is formed as fma(x, c, -M) with M = c ref rounded, which is one
+// instruction less a logit than (x - ref) c; what M's rounding leaves, rho = c ref - M, is taken
+// back batch by batch: 2^-rho s and 2^-rho (u - rho s). That holds for |M| below 1e8 (rho up to
+// 4), and for fp16, whose -inf counts as -65504 there, while 2^((-65504 - ref) c) is 0; beyond,
+// the difference is taken first.
+template <int T>
+struct Running {
+  float m, s, u, ref, M, rho, back;
+  bool small;
+
+  __device__ __forceinline__ void set_ref(float c) {
+    ref = reference(m);
+    M = ref * c;
+    rho = fmaf(ref, c, -M);
+    small = fabsf(M) < 1e8f && (T != TB_FP16 || (ref + 65504.f) * c > 200.f);
+    back = fabsf(rho) < 0x1p-10f ? fmaf(-rho, kLn2, 1.f) : ex2(-rho);
+  }
+  __device__ __forceinline__ void start(float c) {
+    m = -CUDART_INF_F;
+    s = u = 0.f;
+    set_ref(c);
+  }
+  __device__ __forceinline__ void raise(float m2, float c) {
+    move_to(s, u, ref, reference(m2), c);
+    m = m2;
+    set_ref(c);
+  }
+  __device__ __forceinline__ void add(float bs, float bu) {
+    if (small) {
+      bu = back * fmaf(-rho, bs, bu);
+      bs *= back;
+    }
+    s += bs;
+    u += bu;
+  }
+  __device__ __forceinline__ void one(float x, float c) {  // x below m already
+    const float d = (max_nan(x, kLow) - ref) * c, p = ex2(d);
+    s += p;
+    u = fmaf(p, d, u);
+  }
+};
 
 struct FwdArgs {
   const void *logits;
@@ -207,19 +275,20 @@ __device__ __forceinline__ float logprob_of(float x, const State &a, float l, fl
   return kLn2 * fmaf(x - reference(a.m), c, -l);
 }
 
-// One warp writes a row's results. key: the row's list over the lanes.
+// The row's given id and its logit (0 for an id outside).
 template <int T>
+__device__ __forceinline__ float logit_of(const FwdArgs &a, int64_t row, int64_t id) {
+  return id >= 0 && id < a.vocab ? load1<T>(a.logits, row * a.ld + id) : 0.f;
+}
+
+// One warp writes a row's results. key: the row's list over the lanes; x: logit `id`.
 __device__ __forceinline__ void finish_row(const FwdArgs &a, int64_t row, const State &st,
-                                           uint64_t key, int lane) {
+                                           uint64_t key, int64_t id, float x, int lane) {
   const float l = log2f(st.s);
   const bool empty = st.m == -CUDART_INF_F && st.s == st.s;
   if (lane == 0) {
-    const int64_t id = id_of(a.ids, a.ids64, row);
-    float lp = 0.f;
-    if (id >= 0 && id < a.vocab)
-      lp = logprob_of(load1<T>(a.logits, row * a.ld + id), st, l, a.c, a.inv_t);
-    a.logprob[row] = lp;
-    const float h = kLn2 * l - st.u / st.s * a.inv_t;
+    a.logprob[row] = id >= 0 && id < a.vocab ? logprob_of(x, st, l, a.c, a.inv_t) : 0.f;
+    const float h = kLn2 * (l - st.u / st.s);
     a.entropy[row] = empty || h < 0.f ? 0.f : h;
     a.stats[2 * row] = reference(st.m);
     a.stats[2 * row + 1] = empty ? CUDART_INF_F : l;
@@ -231,21 +300,108 @@ __device__ __forceinline__ void finish_row(const FwdArgs &a, int64_t row, const 
   }
 }
 
-__device__ __forceinline__ void add_logit(float x, float ref, float c, float &s, float &u) {
-  const float t = max_nan(x, kLow) - ref;
-  const float p = ex2(t * c);
-  s += p;
-  u = fmaf(p, t, u);
+// The words of a vector held at kLow (fp16: at its lowest value) and above, and their maximum;
+// 16-bit types two at a time.
+template <int T>
+struct Words;
+
+template <>
+struct Words<TB_FP16> {
+  using type = __half2;
+  static __device__ __forceinline__ type low() { return __float2half2_rn(-65504.f); }
+};
+
+template <>
+struct Words<TB_BF16> {
+  using type = __nv_bfloat162;
+  static __device__ __forceinline__ type low() { return __float2bfloat162_rn(kLow); }
+};
+
+template <int T>
+__device__ __forceinline__ uint32_t hold(uint32_t w) {
+  if constexpr (T == TB_FP32) {
+    return __float_as_uint(max_nan(__uint_as_float(w), kLow));
+  } else {
+    using W = typename Words<T>::type;
+    const W v = __hmax2_nan(*reinterpret_cast<W *>(&w), Words<T>::low());
+    return *reinterpret_cast<const uint32_t *>(&v);
+  }
+}
+
+template <int T, int N>
+__device__ __forceinline__ float batch_max(const uint4 (&raw)[N]) {
+  if constexpr (T == TB_FP32) {
+    float m = -CUDART_INF_F;
+#pragma unroll
+    for (int b = 0; b < N; ++b) {
+      m = fmaxf(fmaxf(m, __uint_as_float(raw[b].x)), __uint_as_float(raw[b].y));
+      m = fmaxf(fmaxf(m, __uint_as_float(raw[b].z)), __uint_as_float(raw[b].w));
+    }
+    return m;
+  } else {
+    using W = typename Words<T>::type;
+    uint32_t none = T == TB_FP16 ? 0xfc00fc00u : 0xff80ff80u;  // two -inf
+    W m = *reinterpret_cast<W *>(&none);
+#pragma unroll
+    for (int b = 0; b < N; ++b) {
+      const uint32_t w[4] = {raw[b].x, raw[b].y, raw[b].z, raw[b].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m = __hmax2(m, *reinterpret_cast<const W *>(&w[i]));
+    }
+    const float2 f = Elem<T>::get2(*reinterpret_cast<uint32_t *>(&m));
+    return fmaxf(f.x, f.y);
+  }
 }
 
 template <int T>
-__global__ void __launch_bounds__(kThreads) logprobs_fwd(FwdArgs a) {
+__device__ __forceinline__ void hold_vec(uint4 &v, float (&z)[per_vec<T>()]) {
+  v.x = hold<T>(v.x);
+  v.y = hold<T>(v.y);
+  v.z = hold<T>(v.z);
+  v.w = hold<T>(v.w);
+  unpack_vec<T>(v, z);
+}
+
+template <int T, int N>
+__device__ __forceinline__ void add_batch(Running<T> &r, uint4 (&raw)[N], float c) {
+  constexpr int E = per_vec<T>();
+  float s = 0.f, u = 0.f;
+  if (r.small) {
+#pragma unroll
+    for (int b = 0; b < N; ++b) {
+      float z[E];
+      hold_vec<T>(raw[b], z);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float d = fmaf(z[e], c, -r.M), p = ex2(d);
+        s += p;
+        u = fmaf(p, d, u);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int b = 0; b < N; ++b) {
+      float z[E];
+      unpack_vec<T>(raw[b], z);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float d = (max_nan(z[e], kLow) - r.ref) * c, p = ex2(d);
+        s += p;
+        u = fmaf(p, d, u);
+      }
+    }
+  }
+  r.add(s, u);
+}
+
+template <int T, bool kTop>
+__global__ void __launch_bounds__(kThreads, T == TB_FP32 ? 6 : 5) logprobs_fwd(FwdArgs a) {
   pdl_wait();
   pdl_release();
   constexpr int E = per_vec<T>();
   __shared__ State sh_state[kWarps];
   __shared__ uint64_t sh_list[kWarps][32];
-  __shared__ uint64_t sh_bar;
+  __shared__ float sh_max[kWarps][32];
   __shared__ int sh_n;
   __shared__ uint16_t sh_who[kThreads];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -255,125 +411,102 @@ __global__ void __launch_bounds__(kThreads) logprobs_fwd(FwdArgs a) {
   const int64_t v0 = split * a.split_vecs;
   const int64_t v1 = v0 + a.split_vecs < r.nw ? v0 + a.split_vecs : r.nw;
   const int edges = split == 0 ? r.edges : 0;
-  State st{-CUDART_INF_F, 0.f, 0.f};
-  float ref = reference(st.m);
-  int64_t best = v0 + threadIdx.x;  // first vector of the batch the maximum came from
-  for (int64_t v = v0 + threadIdx.x; v < v1; v += (int64_t)kThreads * kUnroll) {
-    float z[kUnroll][E];
-#pragma unroll
-    for (int b = 0; b < kUnroll; ++b) {
-      const int64_t vb = v + (int64_t)b * kThreads;
-      if (vb < v1) {
-        load_vec<T>(r, vb, z[b]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) z[b][e] = -CUDART_INF_F;
-      }
-    }
-    float m = -CUDART_INF_F;
-#pragma unroll
-    for (int b = 0; b < kUnroll; ++b)
-#pragma unroll
-      for (int e = 0; e < E; ++e) m = fmaxf(m, z[b][e]);
-    if (m > st.m) {
-      move_to(st.s, st.u, ref, reference(m), a.c);
-      ref = reference(m);
-      st.m = m;
-      best = v;
-    }
-#pragma unroll
-    for (int b = 0; b < kUnroll; ++b) {
-      if (v + (int64_t)b * kThreads >= v1) break;
-#pragma unroll
-      for (int e = 0; e < E; ++e) add_logit(z[b][e], ref, a.c, st.s, st.u);
-    }
+  Running<T> run;
+  run.start(a.c);
+  const uint4 *vecs = reinterpret_cast<const uint4 *>(r.base + r.head * elem_size<T>());
+  int64_t v = v0 + threadIdx.x;
+  for (; v + (kUnroll - 1) * kThreads < v1; v += kUnroll * kThreads) {
+    uint4 raw[kUnroll];
+    load_batch(vecs + v, raw);
+    const float m = batch_max<T>(raw);
+    if (m > run.m) run.raise(m, a.c);
+    add_batch<T>(run, raw, a.c);
   }
-  const float own_max = st.m;  // of the whole vectors
+  for (; v < v1; v += kThreads) {
+    uint4 raw[1];
+    load_batch(vecs + v, raw);
+    const float m = batch_max<T>(raw);
+    if (m > run.m) run.raise(m, a.c);
+    add_batch<T>(run, raw, a.c);
+  }
+  const float own_max = run.m;  // of the whole vectors
+  const int64_t id = id_of(a.ids, a.ids64, row);  // used at the end: in flight meanwhile
   uint64_t edge_key = 0;
   if ((int)threadIdx.x < edges) {
     const int64_t col = edge_col<T>(r, threadIdx.x);
     const float x = load1<T>(r.base, col);
     if (x == x) edge_key = make_key(x, col);
-    if (x > st.m) {
-      move_to(st.s, st.u, ref, reference(x), a.c);
-      ref = reference(x);
-      st.m = x;
-    }
-    add_logit(x, ref, a.c, st.s, st.u);
+    if (x > run.m) run.raise(x, a.c);
+    run.one(x, a.c);
   }
-  State w = warp_merge_states(st, a.c);
+  State w = warp_merge_states(State{run.m, run.s, run.u}, a.c);
   if (lane == 0) sh_state[warp] = w;
+  const float x_id = logit_of<T>(a, row, id);
   uint64_t list = 0;
-  if (a.k > 0) {
-    // this thread's largest key among its whole vectors: its maximum's first place
-    uint64_t mine = 0;
-    for (int b = 0; b < kUnroll && mine == 0; ++b) {
-      const int64_t vb = best + (int64_t)b * kThreads;
-      if (vb >= v1) break;
-      float z[E];
-      load_vec<T>(r, vb, z);
-#pragma unroll
-      for (int e = E - 1; e >= 0; --e)
-        if (z[e] == own_max) mine = make_key(z[e], r.head + vb * E + e);
-    }
-    sh_list[warp][lane] = warp_sort(mine, lane);
+  if constexpr (kTop) {
+    // the k-th largest of the threads' maxima; their owners
     if (threadIdx.x == 0) sh_n = 0;
-    __syncthreads();
-    if (warp == 0) {
-      uint64_t top = sh_list[0][lane];
-#pragma unroll
-      for (int i = 1; i < kWarps; ++i) top = warp_merge(top, sh_list[i][lane], lane);
-      top = __shfl_sync(kAll, top, a.k - 1);
-      if (lane == 0) sh_bar = top;
-    }
-    __syncthreads();
-    const uint64_t bar = sh_bar;
-    if (mine != 0 && mine >= bar) sh_who[atomicAdd(&sh_n, 1)] = (uint16_t)threadIdx.x;
+    const bool any_vec = v0 + threadIdx.x < v1;
+    block_merge(warp_sort(any_vec ? own_max : -CUDART_INF_F, lane), sh_max, warp, lane);
+    const float bar = sh_max[0][a.k - 1];
+    if (any_vec && own_max >= bar) sh_who[atomicAdd(&sh_n, 1)] = (uint16_t)threadIdx.x;
     __syncthreads();
     // the owners' vectors once more, and the edges (the first warp holds them all)
-    if (warp == 0) warp_insert(list, edge_key < bar ? 0 : edge_key, a.k, lane);
-    const int64_t each = (v1 - v0 + kThreads - 1) / kThreads;
-    const int64_t items = each * sh_n;
-    for (int64_t i0 = (int64_t)warp * 32; i0 < items; i0 += kThreads) {
-      const int64_t i = i0 + lane;
-      int64_t vb = v1;
-      if (i < items) vb = v0 + sh_who[i / each] + (i % each) * kThreads;
-      float z[E];
-      if (vb < v1) load_vec<T>(r, vb, z);
+    if (warp == 0) warp_insert(list, edge_key, a.k, lane);
+    const int each = (int)((v1 - v0 + kThreads - 1) / kThreads), items = each * sh_n;
+    const int span = (int)(v1 - v0);
+    for (int i0 = warp * 32; i0 < items; i0 += kThreads * kAgain) {
+      uint4 raw[kAgain];
+      int at[kAgain];
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        uint64_t key = 0;
-        if (vb < v1 && z[e] == z[e]) key = make_key(z[e], r.head + vb * E + e);
-        warp_insert(list, key < bar ? 0 : key, a.k, lane);
+      for (int b = 0; b < kAgain; ++b) {
+        const int i = i0 + b * kThreads + lane, who = i / each;
+        at[b] = i < items ? sh_who[who] + (i - who * each) * kThreads : span;
+        if (at[b] < span) raw[b] = __ldg(vecs + v0 + at[b]);
+      }
+#pragma unroll
+      for (int b = 0; b < kAgain; ++b) {
+        float z[E];
+        bool any = false;
+        if (at[b] < span) {
+          unpack_vec<T>(raw[b], z);
+#pragma unroll
+          for (int e = 0; e < E; ++e) any |= z[e] >= bar;
+        }
+        if (__ballot_sync(kAll, any) == 0) continue;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          warp_insert(list, any && z[e] >= bar ? make_key(z[e], r.head + (v0 + at[b]) * E + e) : 0, a.k,
+                      lane);
       }
     }
-    sh_list[warp][lane] = list;  // the maxima were read before the last barrier but one
+    list = block_merge(list, sh_list, warp, lane);
+  } else {
+    __syncthreads();  // sh_state
   }
-  __syncthreads();
   if (warp != 0) return;
   w = lane < kWarps ? sh_state[lane] : State{-CUDART_INF_F, 0.f, 0.f};
   w = warp_merge_states(w, a.c);
-  if (a.k > 0) {
-#pragma unroll
-    for (int i = 1; i < kWarps; ++i) list = warp_merge(list, sh_list[i][lane], lane);
-  }
   if (a.splits == 1) {
-    finish_row<T>(a, row, w, list, lane);
+    finish_row(a, row, w, list, id, x_id, lane);
   } else {
     if (lane == 0) a.states[blockIdx.x] = make_float4(w.m, w.s, w.u, 0.f);
     if (lane < a.k) a.lists[(int64_t)blockIdx.x * a.k + lane] = list;
   }
 }
 
-// A warp per row over its splits' states and lists.
+// A CTA per row over its splits' states and (descending) lists.
 template <int T>
-__global__ void __launch_bounds__(32) logprobs_merge(FwdArgs a) {
+__global__ void __launch_bounds__(kThreads) logprobs_merge(FwdArgs a) {
   pdl_wait();
   pdl_release();
-  const int lane = threadIdx.x;
+  __shared__ uint64_t sh_list[kWarps][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t row = blockIdx.x;
+  const int64_t id = id_of(a.ids, a.ids64, row);
+  const float x_id = logit_of<T>(a, row, id);
   State w{-CUDART_INF_F, 0.f, 0.f};
-  for (int i = lane; i < a.splits; i += 32) {
+  for (int i = lane; i < a.splits && warp == 0; i += 32) {
     const float4 q = a.states[row * a.splits + i];
     State o{q.x, q.y, q.z};
     const float m = fmaxf(w.m, o.m);
@@ -381,14 +514,26 @@ __global__ void __launch_bounds__(32) logprobs_merge(FwdArgs a) {
     move_to(o.s, o.u, reference(o.m), reference(m), a.c);
     w = State{m, w.s + o.s, w.u + o.u};
   }
-  w = warp_merge_states(w, a.c);
   uint64_t list = 0;
-  const int64_t keys = (int64_t)a.splits * a.k;
-  for (int64_t i0 = 0; i0 < keys; i0 += 32) {
-    const int64_t i = i0 + lane;
-    warp_insert(list, i < keys ? a.lists[row * keys + i] : 0, a.k, lane);
+  if (a.k > 0) {
+    constexpr int kAhead = 8;
+    const uint64_t *lists = a.lists + row * a.splits * a.k;
+    for (int i0 = warp; i0 < a.splits; i0 += kWarps * kAhead) {
+      uint64_t key[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const int i = i0 + j * kWarps;
+        key[j] = i < a.splits && lane < a.k ? lists[(int64_t)i * a.k + lane] : 0;
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j)
+        if (i0 + j * kWarps < a.splits) list = warp_merge(list, key[j], lane);
+    }
+    list = block_merge(list, sh_list, warp, lane);
   }
-  finish_row<T>(a, row, w, list, lane);
+  if (warp != 0) return;
+  w = warp_merge_states(w, a.c);
+  finish_row(a, row, w, list, id, x_id, lane);
 }
 
 struct BwdArgs {
@@ -410,6 +555,22 @@ __device__ __forceinline__ float slope(float x, float ref, float l, float c, flo
 }
 
 template <int T>
+__device__ __forceinline__ uint4 slopes(const uint4 &raw, float ref, float l, float c, float A,
+                                        float B) {
+  constexpr int E = per_vec<T>();
+  float z[E];
+  unpack_vec<T>(raw, z);
+#pragma unroll
+  for (int e = 0; e < E; ++e) z[e] = slope(z[e], ref, l, c, A, B);
+  if constexpr (T == TB_FP32)
+    return make_uint4(__float_as_uint(z[0]), __float_as_uint(z[1]), __float_as_uint(z[2]),
+                      __float_as_uint(z[3]));
+  else
+    return make_uint4(Elem<T>::put2(z[0], z[1]), Elem<T>::put2(z[2], z[3]),
+                      Elem<T>::put2(z[4 % E], z[5 % E]), Elem<T>::put2(z[6 % E], z[7 % E]));
+}
+
+template <int T>
 __global__ void __launch_bounds__(kThreads) logprobs_bwd(BwdArgs a) {
   pdl_wait();
   pdl_release();
@@ -420,7 +581,6 @@ __global__ void __launch_bounds__(kThreads) logprobs_bwd(BwdArgs a) {
   const int split = (int)(blockIdx.x - row * a.splits);
   const Row r = row_of<T>(a.logits, row, a.ld, a.vocab);
   char *out = static_cast<char *>(a.grad) + row * a.ld_grad * elem_size<T>();
-  char *out_vecs = out + (int64_t)r.head * elem_size<T>();
   const int64_t v0 = split * a.split_vecs;
   const int64_t v1 = v0 + a.split_vecs < r.nw ? v0 + a.split_vecs : r.nw;
   const int edges = split == 0 ? r.edges : 0;
@@ -444,30 +604,17 @@ __global__ void __launch_bounds__(kThreads) logprobs_bwd(BwdArgs a) {
   const float gh = a.g_ent ? a.g_ent[row] : 0.f;
   const float A = empty ? 0.f : -a.inv_t * (G + gh * a.entropy[row]);
   const float B = empty ? 0.f : -a.inv_t * gh * kLn2;
-  for (int64_t v = v0 + threadIdx.x; v < v1; v += (int64_t)kThreads * kUnroll) {
-    float z[kUnroll][E];
+  const uint4 *vecs = reinterpret_cast<const uint4 *>(r.base + r.head * elem_size<T>());
+  uint4 *out_vecs = reinterpret_cast<uint4 *>(out + r.head * elem_size<T>());
+  int64_t v = v0 + threadIdx.x;
+  for (; v + (kUnroll - 1) * kThreads < v1; v += kUnroll * kThreads) {
+    uint4 raw[kUnroll];
+    load_batch(vecs + v, raw);
 #pragma unroll
-    for (int b = 0; b < kUnroll; ++b) {
-      const int64_t vb = v + (int64_t)b * kThreads;
-      if (vb < v1) load_vec<T>(r, vb, z[b]);
-    }
-#pragma unroll
-    for (int b = 0; b < kUnroll; ++b) {
-      const int64_t vb = v + (int64_t)b * kThreads;
-      if (vb >= v1) break;
-#pragma unroll
-      for (int e = 0; e < E; ++e) z[b][e] = slope(z[b][e], ref, l, a.c, A, B);
-      uint4 w;
-      if constexpr (T == TB_FP32)
-        w = make_uint4(__float_as_uint(z[b][0]), __float_as_uint(z[b][1]),
-                       __float_as_uint(z[b][2]), __float_as_uint(z[b][3]));
-      else
-        w = make_uint4(Elem<T>::put2(z[b][0], z[b][1]), Elem<T>::put2(z[b][2], z[b][3]),
-                       Elem<T>::put2(z[b][4 % E], z[b][5 % E]),
-                       Elem<T>::put2(z[b][6 % E], z[b][7 % E]));
-      *reinterpret_cast<uint4 *>(out_vecs + vb * 16) = w;
-    }
+    for (int b = 0; b < kUnroll; ++b)
+      out_vecs[v + b * kThreads] = slopes<T>(raw[b], ref, l, a.c, A, B);
   }
+  for (; v < v1; v += kThreads) out_vecs[v] = slopes<T>(__ldg(vecs + v), ref, l, a.c, A, B);
   if ((int)threadIdx.x < edges) {
     const int64_t col = edge_col<T>(r, threadIdx.x);
     store1<T>(out, col, slope(load1<T>(r.base, col), ref, l, a.c, A, B));
@@ -485,7 +632,8 @@ __global__ void __launch_bounds__(kThreads) logprobs_bwd(BwdArgs a) {
   }
 }
 
-// Splits of a row: enough CTAs for the device when there are few rows.
+// Splits of a row: four CTAs an SM when there are few rows (621 rows of 151936 fp16: 44 us unsplit,
+// 46 + 3 us for the merge in two, 45 + 3 in four).
 int64_t splits_of(int64_t rows, int64_t vecs, int64_t target) {
   int64_t s = (target + rows - 1) / rows;
   const int64_t most = (vecs + kThreads - 1) / kThreads;
@@ -551,11 +699,14 @@ extern "C" int tb_token_logprobs_fwd(const void *logits, int32_t type, int64_t l
                   (nv + splits - 1) / splits, (int)splits, top_k, ids_int64 != 0,
                   kLog2e / temperature, 1.f / temperature};
   cudaStream_t st = as_stream(stream);
+  const dim3 grid((unsigned)(rows * splits));
   TB_WITH_TYPE(type, T,
-               rc = launch("token_logprobs_fwd", logprobs_fwd<T>, dim3((unsigned)(rows * splits)),
-                           kThreads, 0, st, a);
+               rc = top_k > 0 ? launch("token_logprobs_fwd", logprobs_fwd<T, true>, grid, kThreads,
+                                       0, st, a)
+                              : launch("token_logprobs_fwd", logprobs_fwd<T, false>, grid,
+                                       kThreads, 0, st, a);
                if (rc == TB_OK && splits > 1) rc =
-                   launch("token_logprobs_fwd", logprobs_merge<T>, dim3((unsigned)rows), 32, 0, st,
+                   launch("token_logprobs_fwd", logprobs_merge<T>, dim3((unsigned)rows), kThreads, 0, st,
                           a));
   return rc;
 }
@@ -584,7 +735,7 @@ extern "C" int tb_token_logprobs_bwd(const void *logits, int32_t type, int64_t l
     return set_error(TB_EALIGN, "token_logprobs_bwd: the gradient's rows must lie modulo 16 bytes "
                                 "as the logits' rows do");
   const int64_t nv = most_vecs(vocab, es);
-  const int64_t per = (int64_t)kThreads * kUnroll * 2;
+  const int64_t per = (int64_t)kThreads * kUnroll * 4;
   int64_t splits = (nv + per - 1) / per;
   if (splits > 1024) splits = 1024;
   const BwdArgs a{logits, ids, top_ids, stats, entropy, g_logprob, g_entropy, g_top, grad, rows,

@@ -21,38 +21,36 @@ def counters(n):
     return (int(n) + 3) // 4
 
 
-def _launch(x, residual, out, threshold, scale, seed, offset, state, used):
+def _launch(x, residual, out, threshold, scale, seed, offset, state=None, used=None):
     if x.numel():
-        _lib.call_on(x, "tb_dropout", _lib.ptr(x), _lib.TYPE_CODES[x.dtype], _lib.ptr(residual),
-                     _lib.ptr(out), _lib.TYPE_CODES[out.dtype], x.numel(), threshold, scale, seed,
-                     offset, _lib.ptr(state), _lib.ptr(used), _lib.stream_of(x))
+        _lib.call_on(x, "tb_dropout", x.data_ptr(), _lib.TYPE_CODES[x.dtype], _lib.addr(residual),
+                     out.data_ptr(), _lib.TYPE_CODES[out.dtype], x.numel(), threshold, scale, seed,
+                     offset, _lib.addr(state), _lib.addr(used))
     return out
 
 
 class CounterDropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, threshold, scale, seed, offset, state):
-        ctx.draw = (threshold, scale, seed, offset)
         ctx.dtype = x.dtype
-        used = None
-        if state is not None:
-            # the caller may move its state on before the backward: keep what this call used
-            used = torch.empty(2, dtype=torch.int64, device=x.device)
-            ctx.draw = (threshold, scale, 0, 0)
+        ctx.draw = (threshold, scale, seed, offset)
+        out = torch.empty_like(x if residual is None else residual)
+        if state is None:
+            return _launch(x, residual, out, threshold, scale, seed, offset)
+        # the caller may move its state on before the backward: keep what this call used
+        used = torch.empty_like(state)
         ctx.save_for_backward(used)
-        out = torch.empty(x.shape, dtype=x.dtype if residual is None else residual.dtype,
-                          device=x.device)
+        ctx.draw = (threshold, scale, 0, 0)
         return _launch(x, residual, out, threshold, scale, seed, offset, state, used)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        (used,) = ctx.saved_tensors
         dx = None
         if ctx.needs_input_grad[0]:
             g = dy.contiguous()
-            dx = torch.empty(g.shape, dtype=ctx.dtype, device=g.device)
-            _launch(g, None, dx, *ctx.draw, used, None)
+            dx = torch.empty_like(g, dtype=ctx.dtype)
+            _launch(g, None, dx, *ctx.draw, *ctx.saved_tensors)
         return dx, dy if ctx.needs_input_grad[1] else None, None, None, None, None, None
 
 
@@ -86,5 +84,9 @@ def dropout(x, p, seed, offset=0, residual=None):
     else:
         seed = int(seed) & 0xFFFFFFFFFFFFFFFF
         seed -= (seed >> 63) << 64
-    return CounterDropout.apply(x.contiguous(), residual, round(p * 2 ** 32),
-                                1.0 / (1.0 - p) if p < 1.0 else 0.0, seed, offset, state)
+    x = x.contiguous()
+    threshold, scale = round(p * 2 ** 32), 1.0 / (1.0 - p) if p < 1.0 else 0.0
+    if _lib.needs_grad(x, residual):
+        return CounterDropout.apply(x, residual, threshold, scale, seed, offset, state)
+    return _launch(x, residual, torch.empty_like(x if residual is None else residual), threshold,
+                   scale, seed, offset, state)

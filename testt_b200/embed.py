@@ -23,37 +23,39 @@ def _check_ids(ids, what):
 
 def _grad(ids, dy, dw, scale, padding_idx, accumulate):
     n, (vocab, hidden) = ids.numel(), dw.shape
-    nbytes = _lib.load().tb_embedding_grad_workspace(n, hidden)
-    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dw.device)
-    _lib.call_on(dw, "tb_embedding_grad", _lib.ptr(ids), int(ids.dtype == torch.int64),
-                 _lib.ptr(dy), _lib.TYPE_CODES[dy.dtype], _lib.ptr(dw), _lib.TYPE_CODES[dw.dtype],
-                 scale, padding_idx, int(accumulate), n, hidden, vocab, _lib.ptr(ws), nbytes,
-                 _lib.stream_of(dw))
+    nbytes = _lib.workspace_bytes(dw, "tb_embedding_grad_workspace", n, hidden)
+    ws = dw.new_empty(max(nbytes, 16), dtype=torch.uint8)
+    _lib.call_on(dw, "tb_embedding_grad", ids.data_ptr(), int(ids.dtype == torch.int64),
+                 dy.data_ptr(), _lib.TYPE_CODES[dy.dtype], dw.data_ptr(),
+                 _lib.TYPE_CODES[dw.dtype], scale, padding_idx, int(accumulate), n, hidden, vocab,
+                 ws.data_ptr(), nbytes)
     return dw
+
+
+def _forward(ids, weight, scale, out_dtype):
+    vocab, hidden = weight.shape
+    out = weight.new_empty((*ids.shape, hidden), dtype=out_dtype)
+    if ids.numel():
+        _lib.call_on(weight, "tb_embedding_fwd", ids.data_ptr(), int(ids.dtype == torch.int64),
+                     weight.data_ptr(), _lib.TYPE_CODES[weight.dtype],
+                     weight.stride(0) if vocab > 1 else hidden, out.data_ptr(),
+                     _lib.TYPE_CODES[out_dtype], scale, ids.numel(), hidden, vocab)
+    return out
 
 
 class ScaledEmbedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, weight, scale, padding_idx, out_dtype):
-        vocab, hidden = weight.shape
-        n = ids.numel()
-        out = torch.empty((*ids.shape, hidden), dtype=out_dtype, device=weight.device)
-        if n:
-            _lib.call_on(weight, "tb_embedding_fwd", _lib.ptr(ids), int(ids.dtype == torch.int64),
-                         _lib.ptr(weight), _lib.TYPE_CODES[weight.dtype],
-                         weight.stride(0) if vocab > 1 else hidden, _lib.ptr(out),
-                         _lib.TYPE_CODES[out_dtype], scale, n, hidden, vocab,
-                         _lib.stream_of(weight))
         ctx.save_for_backward(ids)
         ctx.rest = (weight.shape, weight.dtype, scale, padding_idx)
-        return out
+        return _forward(ids, weight, scale, out_dtype)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         (ids,) = ctx.saved_tensors
         shape, dtype, scale, padding_idx = ctx.rest
-        dw = torch.empty(shape, dtype=dtype, device=dy.device)
+        dw = dy.new_empty(shape, dtype=dtype)
         return None, _grad(ids, dy.contiguous(), dw, scale, padding_idx, False), None, None, None
 
 
@@ -75,8 +77,10 @@ def embedding(ids, weight, scale=1.0, padding_idx=None, out_dtype=None):
         raise ValueError(f"embedding: padding_idx {padding_idx} outside [0, {weight.shape[0]})")
     if weight.stride(1) != 1 or (weight.shape[0] > 1 and weight.stride(0) < weight.shape[1]):
         weight = weight.contiguous()
-    return ScaledEmbedding.apply(ids, weight, float(scale),
-                                 -1 if padding_idx is None else int(padding_idx), out_dtype)
+    if _lib.needs_grad(weight):
+        return ScaledEmbedding.apply(ids, weight, float(scale),
+                                     -1 if padding_idx is None else int(padding_idx), out_dtype)
+    return _forward(ids, weight, float(scale), out_dtype)
 
 
 def embedding_grad(ids, dy, vocab, scale=1.0, padding_idx=None, out=None, dtype=None):

@@ -40,25 +40,30 @@ def _grad_like(logits):
     return flat.as_strided((rows, vocab), (ld, 1), lead)
 
 
+def _forward(logits, ids, top_k, temperature):
+    """(logprob, entropy, top_lp, top_ids) and the backward's statistics."""
+    rows, vocab = logits.shape
+    code = _lib.TYPE_CODES[logits.dtype]
+    logprob = logits.new_empty(rows, dtype=torch.float32)
+    entropy = torch.empty_like(logprob)
+    stats = logprob.new_empty((rows, 2))
+    top_lp = logprob.new_empty((rows, top_k))
+    top_ids = logits.new_empty((rows, top_k), dtype=torch.int64)
+    if rows:
+        nbytes = _lib.workspace_bytes(logits, "tb_token_logprobs_workspace", rows, vocab, code,
+                                      top_k)
+        ws = logits.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+        _lib.call_on(logits, "tb_token_logprobs_fwd", logits.data_ptr(), code, _ld(logits),
+                     ids.data_ptr(), int(ids.dtype == torch.int64), temperature, top_k,
+                     logprob.data_ptr(), entropy.data_ptr(), top_lp.data_ptr(), top_ids.data_ptr(),
+                     stats.data_ptr(), rows, vocab, _lib.addr(ws), nbytes)
+    return logprob, entropy, top_lp, top_ids, stats
+
+
 class TokenLogprobsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, ids, top_k, temperature):
-        rows, vocab = logits.shape
-        dev, code = logits.device, _lib.TYPE_CODES[logits.dtype]
-        logprob = torch.empty(rows, dtype=torch.float32, device=dev)
-        entropy = torch.empty(rows, dtype=torch.float32, device=dev)
-        top_lp = torch.empty((rows, top_k), dtype=torch.float32, device=dev)
-        top_ids = torch.empty((rows, top_k), dtype=torch.int64, device=dev)
-        stats = torch.empty((rows, 2), dtype=torch.float32, device=dev)
-        if rows:
-            with torch.cuda.device(dev):
-                nbytes = _lib.load().tb_token_logprobs_workspace(rows, vocab, code, top_k)
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-            _lib.call_on(logits, "tb_token_logprobs_fwd", _lib.ptr(logits), code, _ld(logits),
-                         _lib.ptr(ids), int(ids.dtype == torch.int64), temperature, top_k,
-                         _lib.ptr(logprob), _lib.ptr(entropy), _lib.ptr(top_lp),
-                         _lib.ptr(top_ids), _lib.ptr(stats), rows, vocab, _lib.ptr(ws), nbytes,
-                         _lib.stream_of(logits))
+        logprob, entropy, top_lp, top_ids, stats = _forward(logits, ids, top_k, temperature)
         ctx.save_for_backward(logits, ids, top_ids, stats, entropy)
         ctx.rest = (top_k, temperature)
         ctx.set_materialize_grads(False)
@@ -76,12 +81,12 @@ class TokenLogprobsFn(torch.autograd.Function):
         g_lp, g_ent, g_top = (None if g is None else g.contiguous() for g in (g_lp, g_ent, g_top))
         grad = _grad_like(logits)
         if rows:
-            _lib.call_on(logits, "tb_token_logprobs_bwd", _lib.ptr(logits),
-                         _lib.TYPE_CODES[logits.dtype], _ld(logits), _lib.ptr(ids),
-                         int(ids.dtype == torch.int64), temperature, top_k, _lib.ptr(top_ids),
-                         _lib.ptr(stats), _lib.ptr(entropy), _lib.ptr(g_lp), _lib.ptr(g_ent),
-                         _lib.ptr(g_top), _lib.ptr(grad), grad.stride(0) if rows > 1 else vocab,
-                         rows, vocab, _lib.stream_of(logits))
+            _lib.call_on(logits, "tb_token_logprobs_bwd", logits.data_ptr(),
+                         _lib.TYPE_CODES[logits.dtype], _ld(logits), ids.data_ptr(),
+                         int(ids.dtype == torch.int64), temperature, top_k, top_ids.data_ptr(),
+                         stats.data_ptr(), entropy.data_ptr(), _lib.addr(g_lp), _lib.addr(g_ent),
+                         _lib.addr(g_top), grad.data_ptr(), grad.stride(0) if rows > 1 else vocab,
+                         rows, vocab)
         return grad, None, None, None
 
 
@@ -110,7 +115,11 @@ def token_logprobs(logits, ids, top_k=0, temperature=1.0):
     flat = logits.reshape(-1, vocab)
     if flat.stride(1) != 1 or _ld(flat) < vocab:
         flat = flat.contiguous()
-    out = TokenLogprobsFn.apply(flat, ids.reshape(-1).contiguous(), top_k, temperature)
+    ids = ids.reshape(-1).contiguous()
+    if _lib.needs_grad(flat):
+        out = TokenLogprobsFn.apply(flat, ids, top_k, temperature)
+    else:
+        out = _forward(flat, ids, top_k, temperature)[:4]
     if len(lead) == 1:
         return TokenLogprobs(*out)
     return TokenLogprobs(out[0].view(lead), out[1].view(lead), out[2].view(*lead, top_k),

@@ -26,28 +26,31 @@ def _code(t, default):
     return default if t is None else _lib.TYPE_CODES[t.dtype]
 
 
+def _forward(qkv, lora_q, lora_v, q_weight, k_weight, eps, cos, sin, pos_idx, batch, seq, n_heads,
+             n_kv, head_dim, weight_offset):
+    rows = qkv.shape[0]
+    code = _lib.TYPE_CODES[qkv.dtype]
+    q = qkv.new_empty((rows, n_heads, head_dim))
+    k = qkv.new_empty((rows, n_kv, head_dim))
+    v = torch.empty_like(k)
+    if rows:
+        _lib.call_on(qkv, "tb_norm_rope_fwd", qkv.data_ptr(), code, _ld(qkv), _lib.addr(lora_q),
+                     _lib.addr(lora_v), _code(lora_q if lora_q is not None else lora_v, code),
+                     _lib.addr(q_weight), _lib.addr(k_weight),
+                     _code(q_weight if q_weight is not None else k_weight, code), weight_offset,
+                     eps, cos.data_ptr(), sin.data_ptr(), cos.shape[1], pos_idx.data_ptr(),
+                     q.data_ptr(), k.data_ptr(), v.data_ptr(), rows, batch, seq, n_heads, n_kv,
+                     head_dim)
+    return q, k, v
+
+
 class NormRopeTokens(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, qkv, lora_q, lora_v, q_weight, k_weight, eps, cos, sin, pos_idx, batch, seq,
-                n_heads, n_kv, head_dim, weight_offset):
-        rows, dev, dt = qkv.shape[0], qkv.device, qkv.dtype
-        code = _lib.TYPE_CODES[dt]
-        q = torch.empty((rows, n_heads, head_dim), dtype=dt, device=dev)
-        k = torch.empty((rows, n_kv, head_dim), dtype=dt, device=dev)
-        v = torch.empty((rows, n_kv, head_dim), dtype=dt, device=dev)
-        if rows:
-            _lib.call_on(qkv, "tb_norm_rope_fwd", _lib.ptr(qkv), code, _ld(qkv),
-                         _lib.ptr(lora_q), _lib.ptr(lora_v),
-                         _code(lora_q if lora_q is not None else lora_v, code),
-                         _lib.ptr(q_weight), _lib.ptr(k_weight),
-                         _code(q_weight if q_weight is not None else k_weight, code),
-                         weight_offset, eps, _lib.ptr(cos), _lib.ptr(sin), cos.shape[1],
-                         _lib.ptr(pos_idx), _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), rows, batch,
-                         seq, n_heads, n_kv, head_dim, _lib.stream_of(qkv))
+    def forward(ctx, qkv, lora_q, lora_v, q_weight, k_weight, eps, cos, sin, pos_idx, *dims):
         ctx.save_for_backward(qkv, lora_q, q_weight, k_weight, cos, sin, pos_idx)
-        ctx.dims = (eps, batch, seq, n_heads, n_kv, head_dim, weight_offset)
+        ctx.dims = (eps, *dims)
         ctx.set_materialize_grads(False)
-        return q, k, v
+        return _forward(qkv, lora_q, lora_v, q_weight, k_weight, eps, cos, sin, pos_idx, *dims)
 
     @staticmethod
     @once_differentiable
@@ -55,24 +58,22 @@ class NormRopeTokens(torch.autograd.Function):
         qkv, lora_q, q_weight, k_weight, cos, sin, pos_idx = ctx.saved_tensors
         eps, batch, seq, n_heads, n_kv, head_dim, weight_offset = ctx.dims
         need = ctx.needs_input_grad
-        rows, dev = qkv.shape[0], qkv.device
+        rows = qkv.shape[0]
         code = _lib.TYPE_CODES[qkv.dtype]
         grads = [None if g is None else g.contiguous() for g in (grad_q, grad_k, grad_v)]
-        dqkv = torch.empty((rows, (n_heads + 2 * n_kv) * head_dim), dtype=qkv.dtype, device=dev)
+        dqkv = qkv.new_empty((rows, (n_heads + 2 * n_kv) * head_dim))
         dqw = torch.empty_like(q_weight) if need[3] else None
         dkw = torch.empty_like(k_weight) if need[4] else None
         ws, nbytes = None, 0
-        if dqw is not None or dkw is not None:
-            with torch.cuda.device(dev):
-                nbytes = _lib.load().tb_norm_rope_bwd_workspace(rows, head_dim)
-            ws = torch.empty(max(nbytes // 4, 1), dtype=torch.float32, device=dev)
-        _lib.call_on(qkv, "tb_norm_rope_bwd", _lib.ptr(grads[0]), _lib.ptr(grads[1]),
-                     _lib.ptr(grads[2]), _lib.ptr(qkv), code, _ld(qkv), _lib.ptr(lora_q),
-                     _code(lora_q, code), _lib.ptr(q_weight), _lib.ptr(k_weight),
-                     _code(q_weight if q_weight is not None else k_weight, code), weight_offset,
-                     eps, _lib.ptr(cos), _lib.ptr(sin), cos.shape[1], _lib.ptr(pos_idx),
-                     _lib.ptr(dqkv), _lib.ptr(dqw), _lib.ptr(dkw), _lib.ptr(ws), nbytes, rows,
-                     batch, seq, n_heads, n_kv, head_dim, _lib.stream_of(qkv))
+        if need[3] or need[4]:
+            nbytes = _lib.workspace_bytes(qkv, "tb_norm_rope_bwd_workspace", rows, head_dim)
+            ws = cos.new_empty(max(nbytes // 4, 1))
+        _lib.call_on(qkv, "tb_norm_rope_bwd", *(_lib.addr(g) for g in grads), qkv.data_ptr(), code,
+                     _ld(qkv), _lib.addr(lora_q), _code(lora_q, code), _lib.addr(q_weight),
+                     _lib.addr(k_weight), _code(q_weight if q_weight is not None else k_weight, code),
+                     weight_offset, eps, cos.data_ptr(), sin.data_ptr(), cos.shape[1],
+                     pos_idx.data_ptr(), dqkv.data_ptr(), _lib.addr(dqw), _lib.addr(dkw),
+                     _lib.addr(ws), nbytes, rows, batch, seq, n_heads, n_kv, head_dim)
         q_cols, v_start = n_heads * head_dim, (n_heads + n_kv) * head_dim
         return (dqkv if need[0] else None, dqkv[:, :q_cols] if need[1] else None,
                 dqkv[:, v_start:] if need[2] else None, dqw, dkw, None, None, None, None, None,
@@ -105,31 +106,35 @@ def norm_rope_tokens(qkv, lora_q, lora_v, q_weight, k_weight, eps, cos, sin, pos
         raise ValueError(f"norm_rope_tokens: qkv {tuple(qkv.shape)}, expected "
                          f"[rows, {(n_heads + 2 * n_kv) * head_dim}]")
     rows = qkv.shape[0]
-    for name, t, shape in (("lora_q", lora_q, (rows, n_heads * head_dim)),
-                           ("lora_v", lora_v, (rows, n_kv * head_dim)),
-                           ("q_weight", q_weight, (head_dim,)), ("k_weight", k_weight, (head_dim,)),
-                           ("pos_idx", pos_idx, (rows,))):
-        if t is not None and tuple(t.shape) != shape:
-            raise ValueError(f"norm_rope_tokens: {name} {tuple(t.shape)}, expected {shape}")
-    for t in (lora_q, lora_v, q_weight, k_weight):
-        if t is not None and t.dtype not in _lib.TYPE_CODES:
-            raise TypeError(f"norm_rope_tokens: LoRA rows and weights are fp16, bf16 or fp32, "
-                            f"got {t.dtype}")
+    for name, t, *shape in (("lora_q", lora_q, rows, n_heads * head_dim),
+                            ("lora_v", lora_v, rows, n_kv * head_dim),
+                            ("q_weight", q_weight, head_dim), ("k_weight", k_weight, head_dim)):
+        if t is not None:
+            if list(t.shape) != shape:
+                raise ValueError(f"norm_rope_tokens: {name} {tuple(t.shape)}, expected {shape}")
+            if t.dtype not in _lib.TYPE_CODES:
+                raise TypeError(f"norm_rope_tokens: {name} must be fp16, bf16 or fp32, got "
+                                f"{t.dtype}")
+    if pos_idx.dim() != 1 or pos_idx.shape[0] != rows:
+        raise ValueError(f"norm_rope_tokens: pos_idx {tuple(pos_idx.shape)}, expected {(rows,)}")
     if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[0] < seq or cos.shape[1] % 2 or \
             cos.shape[1] > head_dim:
         raise ValueError(f"norm_rope_tokens: tables {tuple(cos.shape)} and {tuple(sin.shape)} for "
                          f"seq {seq}, head_dim {head_dim}")
     if pos_idx.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"norm_rope_tokens: pos_idx must be int64 or int32, got {pos_idx.dtype}")
+    index = qkv.get_device()
     for t in (lora_q, lora_v, q_weight, k_weight, cos, sin, pos_idx):
-        if t is not None and t.device != qkv.device:
+        if t is not None and t.get_device() != index:
             raise ValueError(f"norm_rope_tokens: operands on {t.device} and {qkv.device}")
     if qkv.stride(1) != 1 or _ld(qkv) < qkv.shape[1]:
         qkv = qkv.contiguous()
     lora_q, lora_v = _pair(lora_q, lora_v, qkv.dtype)
     q_weight, k_weight = _pair(q_weight, k_weight, qkv.dtype)
-    return NormRopeTokens.apply(qkv, lora_q, lora_v, q_weight, k_weight, float(eps),
-                                cos.to(torch.float32).contiguous(),
-                                sin.to(torch.float32).contiguous(),
-                                pos_idx.to(torch.int64).contiguous(), int(batch), int(seq),
-                                int(n_heads), int(n_kv), int(head_dim), float(weight_offset))
+    args = (qkv, lora_q, lora_v, q_weight, k_weight, float(eps),
+            cos.to(torch.float32).contiguous(), sin.to(torch.float32).contiguous(),
+            pos_idx.to(torch.int64).contiguous(), int(batch), int(seq), int(n_heads), int(n_kv),
+            int(head_dim), float(weight_offset))
+    if _lib.needs_grad(qkv, lora_q, lora_v, q_weight, k_weight):
+        return NormRopeTokens.apply(*args)
+    return _forward(*args)
