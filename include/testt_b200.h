@@ -568,8 +568,8 @@ int tb_dropout(const void *x, int32_t x_type, const void *residual, void *y, int
  * (weight_offset + weight) (a NULL weight: 1), turned on their first `rot` dims by row
  * pos_idx[token] % seq of cos / sin (fp32 [seq, rot]); v = x. q [rows, n_heads, head_dim], k and
  * v [rows, n_kv, head_dim] in `type`. A token whose position is outside [0, batch * seq) gives
- * zero rows. head_dim (at most 4096) and rot even; multiples of 16 with 16-byte aligned buffers
- * take the vector path. */
+ * zero rows. head_dim (at most 4096) and rot even; multiples of 8 up to 256 with buffers aligned to
+ * four elements (tables to 16 bytes) take the vector path. */
 int tb_norm_rope_fwd(const void *qkv, int32_t type, int64_t ld, const void *lora_q,
                      const void *lora_v, int32_t lora_type, const void *q_weight,
                      const void *k_weight, int32_t weight_type, float weight_offset, float eps,
@@ -591,7 +591,7 @@ int tb_norm_rope_bwd(const void *dq, const void *dk, const void *dv, const void 
                      int32_t n_heads, int32_t n_kv, int32_t head_dim, void *stream);
 
 /* Bytes of workspace tb_norm_rope_bwd needs for the weights' gradients on the current device. */
-int64_t tb_norm_rope_bwd_workspace(int64_t rows, int32_t head_dim);
+int64_t tb_norm_rope_bwd_workspace(int64_t rows, int32_t n_heads, int32_t n_kv, int32_t head_dim);
 
 /* Scaled embedding: out[t] = scale * table[ids[t]] for n ids (int64, or int32 when ids_int64 is 0);
  * table rows `ld` elements apart, in `type`; out [n, hidden] in `type` or TB_FP32, rounded once.
@@ -620,7 +620,7 @@ int64_t tb_embedding_grad_workspace(int64_t n, int64_t hidden);
  * in `type`, rows ld elements apart; ids (int64, or int32 when ids_int64 is 0): logprob[r] =
  * log softmax(logits[r] / temperature)[ids[r]], 0 where ids[r] is outside [0, vocab); entropy[r];
  * top_logprobs / top_ids [rows, top_k] (top_k 0 to 32): the largest, equal ones by the lowest
- * index. stats fp32 [rows, 2] is what the backward needs. A row of -inf only gives logprob -inf
+ * index. stats fp32 [rows, 3] is what the backward needs. A row of -inf only gives logprob -inf
  * and entropy 0; a NaN or +inf makes its row's results NaN (top_ids in range). Temperature 1e-4 to
  * 1e4, rows below 2^21. `workspace`: tb_token_logprobs_workspace bytes, 16-byte aligned. */
 int tb_token_logprobs_fwd(const void *logits, int32_t type, int64_t ld, const void *ids,
@@ -635,9 +635,9 @@ int tb_token_logprobs_fwd(const void *logits, int32_t type, int64_t ld, const vo
  * bytes as the logits' rows do (TB_EALIGN otherwise). */
 int tb_token_logprobs_bwd(const void *logits, int32_t type, int64_t ld, const void *ids,
                           int32_t ids_int64, float temperature, int32_t top_k,
-                          const int64_t *top_ids, const float *stats, const float *entropy,
-                          const float *g_logprob, const float *g_entropy, const float *g_top,
-                          void *grad, int64_t ld_grad, int64_t rows, int64_t vocab, void *stream);
+                          const int64_t *top_ids, const float *stats, const float *g_logprob,
+                          const float *g_entropy, const float *g_top, void *grad, int64_t ld_grad,
+                          int64_t rows, int64_t vocab, void *stream);
 
 /* Bytes of workspace tb_token_logprobs_fwd needs on the current device (0: none). */
 int64_t tb_token_logprobs_workspace(int64_t rows, int64_t vocab, int32_t type, int32_t top_k);

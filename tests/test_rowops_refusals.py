@@ -61,7 +61,8 @@ def test_norm_rope(lib):
     bwd = [P(256)] * 4 + [0, 1024, None, 0, P(256), P(256), 0, 0.0, 1e-6, P(256), P(256), 64,
                           P(256), P(256), P(256), P(256), P(256), 0, 4, 1, 8, 4, 2, 128, None]
     _refuses(lib, "tb_norm_rope_bwd", bwd, TB_EINVAL, b"workspace of 0")
-    assert lib.tb_norm_rope_bwd_workspace(4, 128) == 4 * 2 * 128 * 4
+    assert lib.tb_norm_rope_bwd_workspace(4, 4, 2, 128) >= 2 * 128 * 4
+    assert lib.tb_norm_rope_bwd_workspace(0, 4, 2, 128) == 0
 
 
 def test_embedding(lib):
@@ -91,11 +92,11 @@ def test_token_logprobs(lib):
                              (12, 2 ** 22, TB_EINVAL, b"rows"), (9, None, TB_EINVAL, b"missing"),
                              (15, need - 1, TB_EINVAL, b"workspace"), (0, P(257), TB_EALIGN, b"aligned")):
         _refuses(lib, "tb_token_logprobs_fwd", fwd[:i] + [v] + fwd[i + 1:], code, text)
-    bwd = [P(256), 0, 1000, P(256), 1, 1.0, 0, None, P(256), P(256), P(256), None, None, P(256),
-           1000, 4, 1000, None]
-    _refuses(lib, "tb_token_logprobs_bwd", bwd[:13] + [P(258)] + bwd[14:], TB_EALIGN, b"modulo 16")
-    _refuses(lib, "tb_token_logprobs_bwd", bwd[:14] + [1001] + bwd[15:], TB_EALIGN, b"modulo 16")
-    _refuses(lib, "tb_token_logprobs_bwd", bwd[:14] + [999] + bwd[15:], TB_EINVAL, b"stride")
+    bwd = [P(256), 0, 1000, P(256), 1, 1.0, 0, None, P(256), P(256), None, None, P(256), 1000, 4,
+           1000, None]
+    _refuses(lib, "tb_token_logprobs_bwd", bwd[:12] + [P(258)] + bwd[13:], TB_EALIGN, b"modulo 16")
+    _refuses(lib, "tb_token_logprobs_bwd", bwd[:13] + [1001] + bwd[14:], TB_EALIGN, b"modulo 16")
+    _refuses(lib, "tb_token_logprobs_bwd", bwd[:13] + [999] + bwd[14:], TB_EINVAL, b"stride")
 
 
 def test_gradient_buffer_lies_as_the_logits_do():

@@ -84,14 +84,14 @@ SIGNATURES = {
                          _P, _P, _I64, _I64, _I64, _I32, _I32, _I32, _P],
     "tb_norm_rope_bwd": [_P, _P, _P, _P, _I32, _I64, _P, _I32, _P, _P, _I32, _F, _F, _P, _P, _I32,
                          _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I32, _I32, _I32, _P],
-    "tb_norm_rope_bwd_workspace": [_I64, _I32],
+    "tb_norm_rope_bwd_workspace": [_I64, _I32, _I32, _I32],
     "tb_embedding_fwd": [_P, _I32, _P, _I32, _I64, _P, _I32, _F, _I64, _I64, _I64, _P],
     "tb_embedding_grad": [_P, _I32, _P, _I32, _P, _I32, _F, _I64, _I32, _I64, _I64, _I64, _P, _I64,
                           _P],
     "tb_embedding_grad_workspace": [_I64, _I64],
     "tb_token_logprobs_fwd": [_P, _I32, _I64, _P, _I32, _F, _I32, _P, _P, _P, _P, _P, _I64, _I64,
                               _P, _I64, _P],
-    "tb_token_logprobs_bwd": [_P, _I32, _I64, _P, _I32, _F, _I32, _P, _P, _P, _P, _P, _P, _P, _I64,
+    "tb_token_logprobs_bwd": [_P, _I32, _I64, _P, _I32, _F, _I32, _P, _P, _P, _P, _P, _P, _I64,
                               _I64, _I64, _P],
     "tb_token_logprobs_workspace": [_I64, _I64, _I32, _I32],
 }

@@ -288,10 +288,12 @@ __device__ __forceinline__ void finish_row(const FwdArgs &a, int64_t row, const 
   const bool empty = st.m == -CUDART_INF_F && st.s == st.s;
   if (lane == 0) {
     a.logprob[row] = id >= 0 && id < a.vocab ? logprob_of(x, st, l, a.c, a.inv_t) : 0.f;
-    const float h = kLn2 * (l - st.u / st.s);
-    a.entropy[row] = empty || h < 0.f ? 0.f : h;
-    a.stats[2 * row] = reference(st.m);
-    a.stats[2 * row + 1] = empty ? CUDART_INF_F : l;
+    float h = kLn2 * (l - st.u / st.s);
+    h = empty || h < 0.f ? 0.f : h;
+    a.entropy[row] = h;
+    a.stats[3 * row] = reference(st.m);
+    a.stats[3 * row + 1] = empty ? CUDART_INF_F : l;
+    a.stats[3 * row + 2] = h;
   }
   if (lane < a.k) {
     a.top_ids[row * a.k + lane] = key == 0 ? 0 : (int64_t)key_index(key);
@@ -540,7 +542,7 @@ struct BwdArgs {
   const void *logits;
   const void *ids;
   const int64_t *top_ids;
-  const float *stats, *entropy, *g_lp, *g_ent, *g_top;
+  const float *stats, *g_lp, *g_ent, *g_top;
   void *grad;
   int64_t rows, vocab, ld, ld_grad, split_vecs;
   int splits, k;
@@ -598,11 +600,11 @@ __global__ void __launch_bounds__(kThreads) logprobs_bwd(BwdArgs a) {
   __syncthreads();
   float G = 0.f;
   for (int j = 0; j <= a.k; ++j) G += sh_g[j];
-  const float ref = a.stats[2 * row];
-  const bool empty = a.stats[2 * row + 1] == CUDART_INF_F;
-  const float l = empty ? 0.f : a.stats[2 * row + 1];
+  const float ref = a.stats[3 * row];
+  const bool empty = a.stats[3 * row + 1] == CUDART_INF_F;
+  const float l = empty ? 0.f : a.stats[3 * row + 1];
   const float gh = a.g_ent ? a.g_ent[row] : 0.f;
-  const float A = empty ? 0.f : -a.inv_t * (G + gh * a.entropy[row]);
+  const float A = empty ? 0.f : -a.inv_t * (G + gh * a.stats[3 * row + 2]);
   const float B = empty ? 0.f : -a.inv_t * gh * kLn2;
   const uint4 *vecs = reinterpret_cast<const uint4 *>(r.base + r.head * elem_size<T>());
   uint4 *out_vecs = reinterpret_cast<uint4 *>(out + r.head * elem_size<T>());
@@ -714,20 +716,19 @@ extern "C" int tb_token_logprobs_fwd(const void *logits, int32_t type, int64_t l
 extern "C" int tb_token_logprobs_bwd(const void *logits, int32_t type, int64_t ld, const void *ids,
                                      int32_t ids_int64, float temperature, int32_t top_k,
                                      const int64_t *top_ids, const float *stats,
-                                     const float *entropy, const float *g_logprob,
-                                     const float *g_entropy, const float *g_top, void *grad,
-                                     int64_t ld_grad, int64_t rows, int64_t vocab, void *stream) {
+                                     const float *g_logprob, const float *g_entropy,
+                                     const float *g_top, void *grad, int64_t ld_grad, int64_t rows, int64_t vocab, void *stream) {
   int rc = check("token_logprobs_bwd", rows, vocab, ld, type, top_k, temperature);
   if (rc != TB_OK) return rc;
   if (rows == 0) return TB_OK;
-  if (!logits || !ids || !stats || !entropy || !grad || (top_k > 0 && !top_ids))
+  if (!logits || !ids || !stats || !grad || (top_k > 0 && !top_ids))
     return set_error(TB_EINVAL, "token_logprobs_bwd: a buffer is missing");
   if (rows > 1 && ld_grad < vocab)
     return set_error(TB_EINVAL, "token_logprobs_bwd: gradient row stride %lld", (long long)ld_grad);
   const int es = elem_size_of(type);
   if (!aligned(logits, es) || !aligned(ids, ids_int64 ? 8 : 4) || !aligned(top_ids, 8) ||
-      !aligned(stats, 4) || !aligned(entropy, 4) || !aligned(g_logprob, 4) ||
-      !aligned(g_entropy, 4) || !aligned(g_top, 4))
+      !aligned(stats, 4) || !aligned(g_logprob, 4) || !aligned(g_entropy, 4) ||
+      !aligned(g_top, 4))
     return set_error(TB_EALIGN, "token_logprobs_bwd: a buffer is not aligned to its element");
   // each gradient row lies in its 16-byte words as the logits' row does
   if (((reinterpret_cast<uintptr_t>(logits) ^ reinterpret_cast<uintptr_t>(grad)) & 15) != 0 ||
@@ -738,7 +739,7 @@ extern "C" int tb_token_logprobs_bwd(const void *logits, int32_t type, int64_t l
   const int64_t per = (int64_t)kThreads * kUnroll * 4;
   int64_t splits = (nv + per - 1) / per;
   if (splits > 1024) splits = 1024;
-  const BwdArgs a{logits, ids, top_ids, stats, entropy, g_logprob, g_entropy, g_top, grad, rows,
+  const BwdArgs a{logits, ids, top_ids, stats, g_logprob, g_entropy, g_top, grad, rows,
                   vocab, ld, ld_grad, (nv + splits - 1) / splits, (int)splits, top_k,
                   ids_int64 != 0, kLog2e / temperature, 1.f / temperature};
   cudaStream_t st = as_stream(stream);

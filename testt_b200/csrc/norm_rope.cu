@@ -18,71 +18,75 @@
 namespace tb {
 namespace {
 
-constexpr int kMaxThreads = 512;
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr uint32_t kAll = 0xffffffffu;
 
 struct NormDims {
   int64_t rows, ld, slots;  // tokens, elements between qkv rows, batch * seq
   int nh, nkv, d, rot;
-  float eps, w0;
+  float eps, w0, inv_d;
 };
+
+// Four neighbouring values as loaded: 8 bytes of a 16-bit type, 16 of fp32.
+template <int T>
+struct Quad {
+  using type = uint2;
+  static __device__ __forceinline__ void get(const type &v, float (&f)[4]) {
+    const float2 a = Elem<T>::get2(v.x), b = Elem<T>::get2(v.y);
+    f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
+  }
+  static __device__ __forceinline__ type put(const float (&f)[4]) {
+    return make_uint2(Elem<T>::put2(f[0], f[1]), Elem<T>::put2(f[2], f[3]));
+  }
+  static __device__ __forceinline__ type zero() { return make_uint2(0, 0); }
+};
+
+template <>
+struct Quad<TB_FP32> {
+  using type = float4;
+  static __device__ __forceinline__ void get(const type &v, float (&f)[4]) {
+    f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+  }
+  static __device__ __forceinline__ type put(const float (&f)[4]) {
+    return make_float4(f[0], f[1], f[2], f[3]);
+  }
+  static __device__ __forceinline__ type zero() { return make_float4(0.f, 0.f, 0.f, 0.f); }
+};
+
+template <int T>
+__device__ __forceinline__ typename Quad<T>::type load4(const void *p, int64_t i) {
+  return __ldg(reinterpret_cast<const typename Quad<T>::type *>(
+      static_cast<const typename Elem<T>::type *>(p) + i));
+}
+
+template <int T>
+__device__ __forceinline__ void store4(void *p, int64_t i, const float (&f)[4]) {
+  *reinterpret_cast<typename Quad<T>::type *>(static_cast<typename Elem<T>::type *>(p) + i) =
+      Quad<T>::put(f);
+}
 
 // Sum over groups of `lanes` (a power of two) neighbouring lanes; every lane gets the total.
 __device__ __forceinline__ float group_sum(float v, int lanes) {
-  for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
   return v;
 }
 
-// The two 8-dim chunks of a lane: lanes below rot / 16 hold a rotation pair (8 dims of each
-// half), the others two neighbouring chunks of the rest.
+// The two quads of a lane: lanes below rot / 8 hold a rotation's pair (four dims of each half),
+// the others two neighbouring quads of the rest.
 struct Chunks {
   int a, b;
   bool live, turn;
 };
 
 __device__ __forceinline__ Chunks chunks_of(int lane, int d, int rot) {
-  const int pairs = rot / 16;
+  const int pairs = rot / 8;
   Chunks c;
   c.turn = lane < pairs;
-  c.a = c.turn ? lane * 8 : rot + (lane - pairs) * 16;
-  c.b = c.turn ? rot / 2 + lane * 8 : c.a + 8;
-  c.live = lane < d / 16;
+  c.a = c.turn ? lane * 4 : rot + (lane - pairs) * 8;
+  c.b = c.turn ? rot / 2 + lane * 4 : c.a + 4;
+  c.live = lane < d / 8;
   return c;
-}
-
-__device__ __forceinline__ void zero8(float (&f)[8]) {
-#pragma unroll
-  for (int e = 0; e < 8; ++e) f[e] = 0.f;
-}
-
-template <int T>
-__device__ __forceinline__ void add8(const void *p, int64_t i, float (&f)[8]) {
-  float a[8];
-  load8<T>(p, i, a);
-#pragma unroll
-  for (int e = 0; e < 8; ++e) f[e] += a[e];
-}
-
-// The inputs of head row hr (q heads, k heads, v heads) of a token at a lane's chunks.
-template <int T, int L>
-__device__ __forceinline__ void load_head(const void *qkv, const void *lq, const void *lv,
-                                          const NormDims &dm, int64_t tok, int hr,
-                                          const Chunks &ch, float (&x1)[8], float (&x2)[8]) {
-  const int64_t at = tok * dm.ld + (int64_t)hr * dm.d;
-  load8<T>(qkv, at + ch.a, x1);
-  load8<T>(qkv, at + ch.b, x2);
-  const void *l = nullptr;
-  int64_t li = 0;
-  if (hr < dm.nh) {
-    l = lq;
-    li = (tok * dm.nh + hr) * (int64_t)dm.d;
-  } else if (hr >= dm.nh + dm.nkv) {
-    l = lv;
-    li = (tok * dm.nkv + hr - dm.nh - dm.nkv) * (int64_t)dm.d;
-  }
-  if (l != nullptr) {
-    add8<L>(l, li + ch.a, x1);
-    add8<L>(l, li + ch.b, x2);
-  }
 }
 
 // Output (or gradient) row of head row hr: q [rows, nh, d], k and v [rows, nkv, d].
@@ -99,191 +103,251 @@ __device__ __forceinline__ P pick(P q, P k, P v, const NormDims &dm, int64_t tok
 }
 
 template <int T>
-__device__ __forceinline__ void load_weight(const void *w, float w0, int i, float (&f)[8]) {
+__device__ __forceinline__ void load_weight(const void *w, float w0, int i, float (&f)[4]) {
   if (w == nullptr) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = 1.f;
+    for (int e = 0; e < 4; ++e) f[e] = 1.f;
   } else {
-    load8<T>(w, i, f);
+    Quad<T>::get(load4<T>(w, i), f);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] += w0;
+    for (int e = 0; e < 4; ++e) f[e] += w0;
   }
 }
 
-// A group of `lanes` lanes per head row, lane chunks as above; a CTA per token. W: the weights'
-// type, L: the LoRA rows'.
+template <int L>
+__device__ __forceinline__ void add4(const void *p, int64_t i, float (&f)[4]) {
+  float a[4];
+  Quad<L>::get(load4<L>(p, i), a);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) f[e] += a[e];
+}
+
+// The rotation's factors of a token at a lane's quads.
+struct Turn {
+  float c1[4], c2[4], s1[4], s2[4];
+  __device__ __forceinline__ void load(const float *cosv, const float *sinv, int64_t row, int rot,
+                                       const Chunks &ch) {
+    Quad<TB_FP32>::get(load4<TB_FP32>(cosv, row * rot + ch.a), c1);
+    Quad<TB_FP32>::get(load4<TB_FP32>(cosv, row * rot + ch.b), c2);
+    Quad<TB_FP32>::get(load4<TB_FP32>(sinv, row * rot + ch.a), s1);
+    Quad<TB_FP32>::get(load4<TB_FP32>(sinv, row * rot + ch.b), s2);
+  }
+};
+
+// `lanes` lanes per head row, so 32 / lanes head rows at a time to a warp. A warp takes a token
+// and every `parts`-th such group of its head rows, two groups in flight; the rotation's factors
+// are loaded once for them. W: the weights' type, L: the LoRA rows'.
 template <int T, int L, int W>
-__global__ void __launch_bounds__(kMaxThreads)
+__global__ void __launch_bounds__(kThreads, 4)
     norm_rope_fwd(const void *__restrict__ qkv, const void *__restrict__ lq,
                   const void *__restrict__ lv, const void *__restrict__ qw,
                   const void *__restrict__ kw, const float *__restrict__ cosv,
                   const float *__restrict__ sinv, const int64_t *__restrict__ pos_idx, void *q,
-                  void *k, void *v, NormDims dm, FastDiv seq_div, int lanes) {
+                  void *k, void *v, NormDims dm, FastDiv seq_div, FastDiv parts, int lanes) {
   pdl_wait();
   pdl_release();
-  const int lane = threadIdx.x & (lanes - 1), slot = threadIdx.x / lanes;
-  const int per_pass = blockDim.x / lanes, total = dm.nh + 2 * dm.nkv;
+  constexpr int kGroups = 2;
+  const uint32_t unit = blockIdx.x * kWarps + (threadIdx.x >> 5);
+  uint32_t tok32, part;
+  parts.divmod(unit, tok32, part);
+  const int64_t tok = tok32;
+  if (tok >= dm.rows) return;
+  const int lane = threadIdx.x & (lanes - 1), slot = (threadIdx.x & 31) / lanes;
+  const int rows_at_once = 32 / lanes, total = dm.nh + 2 * dm.nkv;
   const Chunks ch = chunks_of(lane, dm.d, dm.rot);
-  const int64_t tok = blockIdx.x;
   const int64_t pos = __ldg(pos_idx + tok);
   const bool inside = pos >= 0 && pos < dm.slots;
-  uint32_t b32 = 0, t32 = 0;
-  if (inside) seq_div.divmod((uint32_t)pos, b32, t32);
-  float c1[8], c2[8], s1[8], s2[8];
-  if (ch.live && ch.turn) {
-    const int64_t at = (int64_t)t32 * dm.rot;
-    load8f(cosv + at + ch.a, c1);
-    load8f(cosv + at + ch.b, c2);
-    load8f(sinv + at + ch.a, s1);
-    load8f(sinv + at + ch.b, s2);
-  }
-  for (int hr0 = 0; hr0 < total; hr0 += per_pass) {
-    const int hr = hr0 + slot;
-    const bool live = ch.live && hr < total;
-    float x1[8], x2[8];
-    zero8(x1);
-    zero8(x2);
-    if (live && inside) load_head<T, L>(qkv, lq, lv, dm, tok, hr, ch, x1, x2);
-    float ss = 0.f;
+  Turn t;
+  bool turned = false;
+  for (int hr0 = part * rows_at_once; hr0 < total; hr0 += kGroups * (int)parts.d * rows_at_once) {
+    float x1[kGroups][4], x2[kGroups][4], r[kGroups];
+    typename Quad<T>::type r1[kGroups], r2[kGroups];
+    int hr[kGroups];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) ss += x1[e] * x1[e] + x2[e] * x2[e];
-    ss = group_sum(ss, lanes);
-    if (!live) continue;
-    if (hr < dm.nh + dm.nkv && inside) {
-      const void *w = hr < dm.nh ? qw : kw;
-      const float r = rsqrtf(ss / (float)dm.d + dm.eps);
-      float w1[8], w2[8];
-      load_weight<W>(w, dm.w0, ch.a, w1);
-      load_weight<W>(w, dm.w0, ch.b, w2);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float n1 = x1[e] * r * w1[e], n2 = x2[e] * r * w2[e];
-        x1[e] = ch.turn ? n1 * c1[e] - n2 * s1[e] : n1;
-        x2[e] = ch.turn ? n2 * c2[e] + n1 * s2[e] : n2;
+    for (int j = 0; j < kGroups; ++j) {
+      hr[j] = hr0 + j * (int)parts.d * rows_at_once + slot;
+      r1[j] = r2[j] = Quad<T>::zero();
+      if (ch.live && hr[j] < total && inside) {
+        const int64_t at = tok * dm.ld + (int64_t)hr[j] * dm.d;
+        r1[j] = load4<T>(qkv, at + ch.a);
+        r2[j] = load4<T>(qkv, at + ch.b);
       }
     }
-    int64_t at;
-    void *dst = pick(q, k, v, dm, tok, hr, at);
-    store8<T>(dst, at + ch.a, x1);
-    store8<T>(dst, at + ch.b, x2);
+    if (!turned && ch.live && ch.turn && inside) {
+      uint32_t b32, t32;
+      seq_div.divmod((uint32_t)pos, b32, t32);
+      t.load(cosv, sinv, t32, dm.rot, ch);
+      turned = true;
+    }
+#pragma unroll
+    for (int j = 0; j < kGroups; ++j) {
+      Quad<T>::get(r1[j], x1[j]);
+      Quad<T>::get(r2[j], x2[j]);
+      const bool isq = hr[j] < dm.nh, isv = hr[j] >= dm.nh + dm.nkv && hr[j] < total;
+      const void *l = isq ? lq : isv ? lv : nullptr;
+      if (l != nullptr && ch.live && inside) {
+        const int64_t li = isq ? (tok * dm.nh + hr[j]) * (int64_t)dm.d
+                               : (tok * dm.nkv + hr[j] - dm.nh - dm.nkv) * (int64_t)dm.d;
+        add4<L>(l, li + ch.a, x1[j]);
+        add4<L>(l, li + ch.b, x2[j]);
+      }
+      float ss = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) ss += x1[j][e] * x1[j][e] + x2[j][e] * x2[j][e];
+      r[j] = rsqrtf(group_sum(ss, lanes) * dm.inv_d + dm.eps);
+    }
+#pragma unroll
+    for (int j = 0; j < kGroups; ++j) {
+      if (!ch.live || hr[j] >= total) continue;
+      if (hr[j] < dm.nh + dm.nkv && inside) {
+        const void *w = hr[j] < dm.nh ? qw : kw;
+        float w1[4], w2[4];
+        load_weight<W>(w, dm.w0, ch.a, w1);
+        load_weight<W>(w, dm.w0, ch.b, w2);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float n1 = x1[j][e] * r[j] * w1[e], n2 = x2[j][e] * r[j] * w2[e];
+          x1[j][e] = ch.turn ? n1 * t.c1[e] - n2 * t.s1[e] : n1;
+          x2[j][e] = ch.turn ? n2 * t.c2[e] + n1 * t.s2[e] : n2;
+        }
+      }
+      int64_t at;
+      void *dst = pick(q, k, v, dm, tok, hr[j], at);
+      store4<T>(dst, at + ch.a, x1[j]);
+      store4<T>(dst, at + ch.b, x2[j]);
+    }
   }
 }
 
-// Backward over tokens blockIdx, + gridDim, ...; part (may be NULL): fp32 [gridDim, 2, d], this
-// CTA's sums of dqw and dkw.
+// Backward. Each warp keeps one group of head rows and walks tokens warp / groups, + stride, ...,
+// the next token's rows in flight while this one's are worked on; so a lane's head row, weights
+// and weight sums stay the same. part (may be NULL): fp32 [gridDim, 2, d], this CTA's sums of dqw
+// and dkw.
 template <int T, int L, int W>
-__global__ void __launch_bounds__(kMaxThreads)
+__global__ void __launch_bounds__(kThreads, 3)
     norm_rope_bwd(const void *__restrict__ dq, const void *__restrict__ dk,
                   const void *__restrict__ dv, const void *__restrict__ qkv,
                   const void *__restrict__ lq, const void *__restrict__ qw,
                   const void *__restrict__ kw, const float *__restrict__ cosv,
                   const float *__restrict__ sinv, const int64_t *__restrict__ pos_idx,
                   void *__restrict__ dqkv, float *__restrict__ part, NormDims dm, FastDiv seq_div,
-                  int lanes) {
+                  int lanes, int groups) {
   pdl_wait();
   pdl_release();
-  const int lane = threadIdx.x & (lanes - 1), slot = threadIdx.x / lanes;
-  const int per_pass = blockDim.x / lanes, total = dm.nh + 2 * dm.nkv;
+  using Raw = typename Quad<T>::type;
+  const int wid = blockIdx.x * kWarps + (threadIdx.x >> 5);
+  const int stride = (int)gridDim.x * kWarps / groups;  // tokens between a warp's
+  const int lane = threadIdx.x & (lanes - 1), slot = (threadIdx.x & 31) / lanes;
+  const int rows_at_once = 32 / lanes, total = dm.nh + 2 * dm.nkv;
+  const int hr = (wid % groups) * rows_at_once + slot;
   const Chunks ch = chunks_of(lane, dm.d, dm.rot);
+  const bool live = ch.live && hr < total, normed = live && hr < dm.nh + dm.nkv;
   const int64_t width = (int64_t)total * dm.d;
-  float aq1[8], aq2[8], ak1[8], ak2[8];
-  zero8(aq1);
-  zero8(aq2);
-  zero8(ak1);
-  zero8(ak2);
-  for (int64_t tok = blockIdx.x; tok < dm.rows; tok += gridDim.x) {
-    const int64_t pos = __ldg(pos_idx + tok);
+  float a1[4] = {0.f, 0.f, 0.f, 0.f}, a2[4] = {0.f, 0.f, 0.f, 0.f};
+  float w1[4], w2[4];
+  if (normed) {
+    load_weight<W>(hr < dm.nh ? qw : kw, dm.w0, ch.a, w1);
+    load_weight<W>(hr < dm.nh ? qw : kw, dm.w0, ch.b, w2);
+  }
+  int64_t tok = wid / groups < stride ? wid / groups : dm.rows;  // warps left over do nothing
+  Raw g1 = Quad<T>::zero(), g2 = g1, x1 = g1, x2 = g1;
+  int64_t pos = -1;
+  auto load = [&](int64_t at_tok) {
+    g1 = g2 = x1 = x2 = Quad<T>::zero();
+    if (at_tok < dm.rows) {
+      pos = __ldg(pos_idx + at_tok);
+      if (live) {
+        int64_t at;
+        const void *src = pick(dq, dk, dv, dm, at_tok, hr, at);
+        if (src != nullptr) {
+          g1 = load4<T>(src, at + ch.a);
+          g2 = load4<T>(src, at + ch.b);
+        }
+      }
+      if (normed) {
+        const int64_t at = at_tok * dm.ld + (int64_t)hr * dm.d;
+        x1 = load4<T>(qkv, at + ch.a);
+        x2 = load4<T>(qkv, at + ch.b);
+      }
+    }
+  };
+  load(tok);
+  for (; tok < dm.rows; tok += stride) {
     const bool inside = pos >= 0 && pos < dm.slots;
     uint32_t b32 = 0, t32 = 0;
     if (inside) seq_div.divmod((uint32_t)pos, b32, t32);
-    float c1[8], c2[8], s1[8], s2[8];
-    if (ch.live && ch.turn) {
-      const int64_t at = (int64_t)t32 * dm.rot;
-      load8f(cosv + at + ch.a, c1);
-      load8f(cosv + at + ch.b, c2);
-      load8f(sinv + at + ch.a, s1);
-      load8f(sinv + at + ch.b, s2);
+    Turn t;
+    if (normed && ch.turn) t.load(cosv, sinv, t32, dm.rot, ch);
+    float f1[4], f2[4], y1[4], y2[4];
+    Quad<T>::get(g1, f1);
+    Quad<T>::get(g2, f2);
+    Quad<T>::get(x1, y1);
+    Quad<T>::get(x2, y2);
+    if (lq != nullptr && live && hr < dm.nh) {
+      const int64_t li = (tok * dm.nh + hr) * (int64_t)dm.d;
+      add4<L>(lq, li + ch.a, y1);
+      add4<L>(lq, li + ch.b, y2);
     }
-    for (int hr0 = 0; hr0 < total; hr0 += per_pass) {
-      const int hr = hr0 + slot;
-      const bool live = ch.live && hr < total;
-      const bool normed = hr < dm.nh + dm.nkv;
-      float g1[8], g2[8], x1[8], x2[8], w1[8], w2[8];
-      zero8(g1);
-      zero8(g2);
-      zero8(x1);
-      zero8(x2);
-      if (live && inside) {
-        int64_t at;
-        const void *src = pick(dq, dk, dv, dm, tok, hr, at);
-        if (src != nullptr) {
-          load8<T>(src, at + ch.a, g1);
-          load8<T>(src, at + ch.b, g2);
-        }
-        if (normed) {
-          load_head<T, L>(qkv, lq, nullptr, dm, tok, hr, ch, x1, x2);
-          const void *w = hr < dm.nh ? qw : kw;
-          load_weight<W>(w, dm.w0, ch.a, w1);
-          load_weight<W>(w, dm.w0, ch.b, w2);
-        }
-      }
-      float ss = 0.f, gx = 0.f;
-      if (live && normed && inside) {
+    load(tok + stride);
+    float ss = 0.f, gx = 0.f;
+    if (normed) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (ch.turn) {
-            const float d1 = g1[e] * c1[e] + g2[e] * s2[e];
-            const float d2 = g2[e] * c2[e] - g1[e] * s1[e];
-            g1[e] = d1;
-            g2[e] = d2;
-          }
-          ss += x1[e] * x1[e] + x2[e] * x2[e];
-          gx += g1[e] * w1[e] * x1[e] + g2[e] * w2[e] * x2[e];
+      for (int e = 0; e < 4; ++e) {
+        if (ch.turn) {
+          const float d1 = f1[e] * t.c1[e] + f2[e] * t.s2[e];
+          const float d2 = f2[e] * t.c2[e] - f1[e] * t.s1[e];
+          f1[e] = d1;
+          f2[e] = d2;
         }
+        ss += y1[e] * y1[e] + y2[e] * y2[e];
+        gx += f1[e] * w1[e] * y1[e] + f2[e] * w2[e] * y2[e];
       }
-      ss = group_sum(ss, lanes);
-      gx = group_sum(gx, lanes);
-      if (!live) continue;
-      if (normed && inside) {
-        const float r = rsqrtf(ss / (float)dm.d + dm.eps);
-        const float k2 = r * r * (gx / (float)dm.d);
-        const bool isq = hr < dm.nh;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float p1 = g1[e] * x1[e] * r, p2 = g2[e] * x2[e] * r;
-          aq1[e] += isq ? p1 : 0.f;
-          aq2[e] += isq ? p2 : 0.f;
-          ak1[e] += isq ? 0.f : p1;
-          ak2[e] += isq ? 0.f : p2;
-          g1[e] = r * (g1[e] * w1[e] - x1[e] * k2);
-          g2[e] = r * (g2[e] * w2[e] - x2[e] * k2);
-        }
-      }
-      const int64_t at = tok * width + (int64_t)hr * dm.d;
-      store8<T>(dqkv, at + ch.a, g1);
-      store8<T>(dqkv, at + ch.b, g2);
     }
+    ss = group_sum(ss, lanes);
+    gx = group_sum(gx, lanes);
+    if (!live) continue;
+    if (!inside) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f1[e] = f2[e] = 0.f;
+    } else if (normed) {
+      const float r = rsqrtf(ss * dm.inv_d + dm.eps);
+      const float k2 = r * r * (gx * dm.inv_d);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        a1[e] += f1[e] * y1[e] * r;
+        a2[e] += f2[e] * y2[e] * r;
+        f1[e] = r * (f1[e] * w1[e] - y1[e] * k2);
+        f2[e] = r * (f2[e] * w2[e] - y2[e] * k2);
+      }
+    }
+    const int64_t at = tok * width + (int64_t)hr * dm.d;
+    store4<T>(dqkv, at + ch.a, f1);
+    store4<T>(dqkv, at + ch.b, f2);
   }
   if (part == nullptr) return;
-  // the head groups' sums, added in order of the group: first dqw's, then dkw's
-  extern __shared__ float sums[];  // [per_pass][d]
+  // the lanes' sums, added in order of the warps and their head rows
+  __shared__ float sums[kThreads][8];
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    if (half) __syncthreads();
-    if (ch.live) {
-      float *mine = sums + slot * dm.d;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        mine[ch.a + e] = half ? ak1[e] : aq1[e];
-        mine[ch.b + e] = half ? ak2[e] : aq2[e];
+  for (int e = 0; e < 4; ++e) {
+    sums[threadIdx.x][e] = a1[e];
+    sums[threadIdx.x][4 + e] = a2[e];
+  }
+  __syncthreads();
+  const int pairs = dm.rot / 8;
+  for (int i = threadIdx.x; i < 2 * dm.d; i += kThreads) {
+    const int dim = i < dm.d ? i : i - dm.d, h = dm.rot / 2;
+    const int rest = dim - dm.rot;
+    const int at = dim < dm.rot ? (dim % h) / 4 : pairs + rest / 8;
+    const int e = dim < dm.rot ? (dim >= h ? 4 : 0) + dim % 4 : rest % 8;
+    float s = 0.f;
+    for (int w = 0; w < kWarps; ++w) {
+      const int first = ((blockIdx.x * kWarps + w) % groups) * rows_at_once;
+      for (int j = 0; j < rows_at_once; ++j) {
+        const bool isq = first + j < dm.nh, isk = !isq && first + j < dm.nh + dm.nkv;
+        if (i < dm.d ? isq : isk) s += sums[w * 32 + j * lanes + at][e];
       }
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < dm.d; i += blockDim.x) {
-      float s = 0.f;
-      for (int j = 0; j < per_pass; ++j) s += sums[j * dm.d + i];
-      part[((int64_t)blockIdx.x * 2 + half) * dm.d + i] = s;
-    }
+    part[(int64_t)blockIdx.x * 2 * dm.d + i] = s;
   }
 }
 
@@ -339,7 +403,7 @@ __global__ void __launch_bounds__(256)
         const float x = load_x<T>(qkv, l, l_type, at, out, i);
         ss += x * x;
       }
-    const float r = rsqrtf(warp_sum(ss) / (float)dm.d + dm.eps);
+    const float r = rsqrtf(warp_sum(ss) * dm.inv_d + dm.eps);
     const void *w = hr < dm.nh ? qw : kw;
     for (int j = lane; j < dm.d / 2; j += 32) {
       int a, b;
@@ -396,8 +460,8 @@ __global__ void __launch_bounds__(32)
       for (int phase = normed && inside ? 0 : 1; phase < 2; ++phase) {
         float r = 0.f, k2 = 0.f;
         if (phase == 1) {
-          r = rsqrtf(warp_sum(ss) / (float)dm.d + dm.eps);
-          k2 = r * r * (warp_sum(gx) / (float)dm.d);
+          r = rsqrtf(warp_sum(ss) * dm.inv_d + dm.eps);
+          k2 = r * r * (warp_sum(gx) * dm.inv_d);
         }
         for (int j = lane; j < dm.d / 2; j += 32) {
           int a, b;
@@ -443,23 +507,26 @@ __global__ void __launch_bounds__(32)
   }
 }
 
-// dqw / dkw from the CTAs' sums: 32 columns a block, 8 groups of CTAs each in order, then the
+// dqw / dkw from the CTAs' sums: 32 columns a block, 32 groups of CTAs each in order, then the
 // groups in order.
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(1024)
     norm_rope_dw(const float *__restrict__ part, int ctas, int d, void *dqw, void *dkw,
                  int w_type) {
   pdl_wait();
   pdl_release();
-  __shared__ float sh[8][33];
-  const int col = blockIdx.x * 32 + (threadIdx.x & 31), grp = threadIdx.x >> 5;
-  const int per = (ctas + 7) / 8;
+  __shared__ float sh[32][33];
+  const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
+  const int per = (ctas + 31) / 32;
   float s = 0.f;
-  if (col < 2 * d)
-    for (int c = grp * per; c < (grp + 1) * per && c < ctas; ++c) s += part[(int64_t)c * 2 * d + col];
-  sh[grp][threadIdx.x & 31] = s;
+  if (col < 2 * d) {
+#pragma unroll 8
+    for (int c = grp * per; c < (grp + 1) * per; ++c)
+      s += c < ctas ? part[(int64_t)c * 2 * d + col] : 0.f;
+  }
+  sh[grp][lane] = s;
   __syncthreads();
   if (grp != 0 || col >= 2 * d) return;
-  for (int g = 1; g < 8; ++g) s += sh[g][threadIdx.x];
+  for (int g = 1; g < 32; ++g) s += sh[g][lane];
   void *dst = col < d ? dqw : dkw;
   if (dst == nullptr) return;
   TB_WITH_TYPE(w_type, T, store1<T>(dst, col < d ? col : col - d, s));
@@ -473,20 +540,32 @@ int pow2_at_least(int n) {
 
 // Lanes of a head row on the vector path (0: not taken).
 int lanes_of(const NormDims &dm) {
-  if (dm.d % 16 || dm.rot % 16 || dm.d > 512) return 0;
-  return pow2_at_least(dm.d / 16);
+  if (dm.d % 8 || dm.rot % 8 || dm.d > 256) return 0;
+  return pow2_at_least(dm.d / 8);
 }
 
-int threads_of(const NormDims &dm, int lanes) {
-  int t = (dm.nh + 2 * dm.nkv) * lanes;
-  t = (t + 31) / 32 * 32;
-  return t > kMaxThreads ? kMaxThreads : t;
+int groups_of(const NormDims &dm, int lanes) {
+  const int at_once = 32 / lanes;
+  return (dm.nh + 2 * dm.nkv + at_once - 1) / at_once;
 }
 
-// CTAs of the backward: two waves' worth at most, so that a CTA's weight sums cover many tokens.
-int bwd_ctas(int64_t rows) {
-  const int64_t cap = (int64_t)sm_count() * 4;
-  return (int)(rows < cap ? rows : cap);
+// Warps a token's head rows are spread over in the forward: one when there are many tokens.
+int parts_of(const NormDims &dm, int groups) {
+  const int64_t want = ((int64_t)sm_count() * 32 + dm.rows - 1) / dm.rows;
+  return (int)(want < groups ? want : groups);
+}
+
+// CTAs of the backward: at most the resident ones, whose warps walk the tokens (the vector kernel:
+// at least a warp for each group of head rows; the other: one warp a CTA).
+int bwd_ctas(int64_t rows, int groups) {
+  if (groups == 0) {
+    const int64_t cap = (int64_t)sm_count() * 8;
+    return (int)(rows < cap ? rows : cap);
+  }
+  int64_t cap = (int64_t)sm_count() * 3;
+  if (cap < (groups + kWarps - 1) / kWarps) cap = (groups + kWarps - 1) / kWarps;
+  const int64_t want = (rows * groups + kWarps - 1) / kWarps;
+  return (int)(want < cap ? want : cap);
 }
 
 int check(const char *what, const NormDims &dm, int64_t batch, int64_t seq, int type, int l_type,
@@ -527,7 +606,8 @@ extern "C" int tb_norm_rope_fwd(const void *qkv, int32_t type, int64_t ld, const
                                 const int64_t *pos_idx, void *q, void *k, void *v, int64_t rows,
                                 int64_t batch, int64_t seq, int32_t n_heads, int32_t n_kv,
                                 int32_t head_dim, void *stream) {
-  NormDims dm{rows, ld, batch * seq, n_heads, n_kv, head_dim, rot, eps, weight_offset};
+  NormDims dm{rows, ld, batch * seq, n_heads, n_kv, head_dim, rot, eps, weight_offset,
+              1.f / (float)(head_dim > 0 ? head_dim : 1)};
   int rc = check("norm_rope_fwd", dm, batch, seq, type, lora_type, weight_type);
   if (rc != TB_OK) return rc;
   if (rows == 0) return TB_OK;
@@ -538,17 +618,21 @@ extern "C" int tb_norm_rope_fwd(const void *qkv, int32_t type, int64_t ld, const
       !all_aligned({q_weight, k_weight}, ws) || !all_aligned({cos, sin}, 4) || !aligned(pos_idx, 8))
     return set_error(TB_EALIGN, "norm_rope_fwd: a buffer is not aligned to its element");
   const int lanes = lanes_of(dm);
-  const bool vec = lanes > 0 && ld * es % 16 == 0 &&
-                   all_aligned({qkv, q, k, v, lora_q, lora_v, q_weight, k_weight, cos, sin}, 16);
+  const bool vec = lanes > 0 && ld % 4 == 0 && all_aligned({qkv, q, k, v}, 4 * es) &&
+                   all_aligned({lora_q, lora_v}, 4 * ls) &&
+                   all_aligned({q_weight, k_weight}, 4 * ws) && all_aligned({cos, sin}, 16);
   cudaStream_t st = as_stream(stream);
   // the LoRA rows and the weights in qkv's type or fp32 on the vector path
-  const bool l_own = lora_type == type || (!lora_q && !lora_v), w_own = weight_type == type || (!q_weight && !k_weight);
+  const bool l_own = lora_type == type || (!lora_q && !lora_v);
+  const bool w_own = weight_type == type || (!q_weight && !k_weight);
   if (vec && (l_own || lora_type == TB_FP32) && (w_own || weight_type == TB_FP32)) {
     const FastDiv sd((uint32_t)seq);
+    const int parts = parts_of(dm, groups_of(dm, lanes));
+    const int64_t ctas = (rows * parts + kWarps - 1) / kWarps;
 #define TB_FWD(T, L, W)                                                                          \
-  return launch("norm_rope_fwd", norm_rope_fwd<T, L, W>, dim3((unsigned)rows),                   \
-                threads_of(dm, lanes), 0, st, qkv, lora_q, lora_v, q_weight, k_weight, cos, sin, \
-                pos_idx, q, k, v, dm, sd, lanes)
+  return launch("norm_rope_fwd", norm_rope_fwd<T, L, W>, dim3((unsigned)ctas),                   \
+                kThreads, 0, st, qkv, lora_q, lora_v, q_weight, k_weight, cos, sin, pos_idx, q,  \
+                k, v, dm, sd, FastDiv((uint32_t)parts), lanes)
     if (l_own && w_own) TB_WITH_TYPE(type, T, TB_FWD(T, T, T));
     if (l_own) TB_WITH_TYPE(type, T, TB_FWD(T, T, TB_FP32));
     if (w_own) TB_WITH_TYPE(type, T, TB_FWD(T, TB_FP32, T));
@@ -564,9 +648,13 @@ extern "C" int tb_norm_rope_fwd(const void *qkv, int32_t type, int64_t ld, const
                              cos, sin, pos_idx, q, k, v, dm, seq));
 }
 
-extern "C" int64_t tb_norm_rope_bwd_workspace(int64_t rows, int32_t head_dim) {
-  if (rows <= 0 || head_dim <= 0) return 0;
-  return (int64_t)bwd_ctas(rows) * 2 * head_dim * 4;
+extern "C" int64_t tb_norm_rope_bwd_workspace(int64_t rows, int32_t n_heads, int32_t n_kv,
+                                              int32_t head_dim) {
+  if (rows <= 0 || n_heads <= 0 || n_kv < 0 || head_dim <= 0) return 0;
+  const NormDims dm{rows, 0, 0, n_heads, n_kv, head_dim, 0, 0.f, 0.f, 0.f};
+  const int lanes = lanes_of(dm);
+  const int vec = lanes > 0 ? bwd_ctas(rows, groups_of(dm, lanes)) : 0, any = bwd_ctas(rows, 0);
+  return (int64_t)(vec > any ? vec : any) * 2 * head_dim * 4;
 }
 
 extern "C" int tb_norm_rope_bwd(const void *dq, const void *dk, const void *dv, const void *qkv,
@@ -577,7 +665,8 @@ extern "C" int tb_norm_rope_bwd(const void *dq, const void *dk, const void *dv, 
                                 void *dk_weight, void *workspace, int64_t workspace_bytes,
                                 int64_t rows, int64_t batch, int64_t seq, int32_t n_heads,
                                 int32_t n_kv, int32_t head_dim, void *stream) {
-  NormDims dm{rows, ld, batch * seq, n_heads, n_kv, head_dim, rot, eps, weight_offset};
+  NormDims dm{rows, ld, batch * seq, n_heads, n_kv, head_dim, rot, eps, weight_offset,
+              1.f / (float)(head_dim > 0 ? head_dim : 1)};
   int rc = check("norm_rope_bwd", dm, batch, seq, type, lora_type, weight_type);
   if (rc != TB_OK) return rc;
   const bool want_dw = dq_weight || dk_weight;
@@ -590,32 +679,35 @@ extern "C" int tb_norm_rope_bwd(const void *dq, const void *dk, const void *dv, 
       !all_aligned({cos, sin, workspace}, 4) || !aligned(pos_idx, 8))
     return set_error(TB_EALIGN, "norm_rope_bwd: a buffer is not aligned to its element");
   if (want_dw && rows > 0 &&
-      (!workspace || workspace_bytes < tb_norm_rope_bwd_workspace(rows, head_dim)))
+      (!workspace || workspace_bytes < tb_norm_rope_bwd_workspace(rows, n_heads, n_kv, head_dim)))
     return set_error(TB_EINVAL, "norm_rope_bwd: workspace of %lld bytes, %lld needed",
                      (long long)workspace_bytes,
-                     (long long)tb_norm_rope_bwd_workspace(rows, head_dim));
+                     (long long)tb_norm_rope_bwd_workspace(rows, n_heads, n_kv, head_dim));
   float *part = want_dw ? static_cast<float *>(workspace) : nullptr;
   cudaStream_t st = as_stream(stream);
-  const int ctas = rows > 0 ? bwd_ctas(rows) : 0;
+  int ctas = 0;
   if (rows > 0) {
     const int lanes = lanes_of(dm);
-    const bool vec = lanes > 0 && ld * es % 16 == 0 &&
-                     all_aligned({qkv, dq, dk, dv, dqkv, lora_q, q_weight, k_weight, cos, sin}, 16);
-    const bool l_own = lora_type == type || !lora_q, w_own = weight_type == type || (!q_weight && !k_weight);
+    const bool vec = lanes > 0 && ld % 4 == 0 && all_aligned({qkv, dq, dk, dv, dqkv}, 4 * es) &&
+                     aligned(lora_q, 4 * ls) && all_aligned({q_weight, k_weight}, 4 * ws) &&
+                     all_aligned({cos, sin}, 16);
+    const bool l_own = lora_type == type || !lora_q;
+    const bool w_own = weight_type == type || (!q_weight && !k_weight);
     if (vec && (l_own || lora_type == TB_FP32) && (w_own || weight_type == TB_FP32)) {
       const FastDiv sd((uint32_t)seq);
-      const int threads = threads_of(dm, lanes);
-      const size_t smem = part ? (size_t)(threads / lanes) * head_dim * 4 : 0;  // 32 KB at most
+      const int groups = groups_of(dm, lanes);
+      ctas = bwd_ctas(rows, groups);
 #define TB_BWD(T, L, W)                                                                          \
-  rc = launch("norm_rope_bwd", norm_rope_bwd<T, L, W>, dim3((unsigned)ctas), threads, smem, st,  \
-              dq, dk, dv, qkv, lora_q, q_weight, k_weight, cos, sin, pos_idx, dqkv, part, dm, sd, \
-              lanes)
+  rc = launch("norm_rope_bwd", norm_rope_bwd<T, L, W>, dim3((unsigned)ctas), kThreads, 0, st, dq, \
+              dk, dv, qkv, lora_q, q_weight, k_weight, cos, sin, pos_idx, dqkv, part, dm, sd,     \
+              lanes, groups)
       if (l_own && w_own) TB_WITH_TYPE(type, T, TB_BWD(T, T, T));
       else if (l_own) TB_WITH_TYPE(type, T, TB_BWD(T, T, TB_FP32));
       else if (w_own) TB_WITH_TYPE(type, T, TB_BWD(T, TB_FP32, T));
       else TB_WITH_TYPE(type, T, TB_BWD(T, TB_FP32, TB_FP32));
 #undef TB_BWD
     } else {
+      ctas = bwd_ctas(rows, 0);
       TB_WITH_TYPE(type, T,
                    rc = launch("norm_rope_bwd", norm_rope_bwd_any<T>, dim3((unsigned)ctas), 32,
                                (size_t)2 * head_dim * 4, st, dq, dk, dv, qkv, lora_q, lora_type,
@@ -625,6 +717,6 @@ extern "C" int tb_norm_rope_bwd(const void *dq, const void *dk, const void *dv, 
     if (rc != TB_OK) return rc;
   }
   if (!want_dw) return TB_OK;
-  return launch("norm_rope_dw", norm_rope_dw, dim3((unsigned)((2 * head_dim + 31) / 32)), 256, 0,
+  return launch("norm_rope_dw", norm_rope_dw, dim3((unsigned)((2 * head_dim + 31) / 32)), 1024, 0,
                 st, part, ctas, head_dim, dq_weight, dk_weight, weight_type);
 }

@@ -33,6 +33,8 @@ def _grad_like(logits):
     """An empty gradient whose rows lie modulo 16 bytes as the logits' rows do, so that both are
     read and written in whole 16-byte words (at most 7 spare columns a row)."""
     rows, vocab = logits.shape
+    if logits.is_contiguous() and logits.data_ptr() % 16 == 0:
+        return torch.empty_like(logits)
     per = 16 // logits.element_size()
     ld = vocab + (_ld(logits) - vocab) % per
     lead = logits.data_ptr() % 16 // logits.element_size()
@@ -41,22 +43,24 @@ def _grad_like(logits):
 
 
 def _forward(logits, ids, top_k, temperature):
-    """(logprob, entropy, top_lp, top_ids) and the backward's statistics."""
+    """(logprob, entropy, top_lp, top_ids) and the buffer that ends with the backward's
+    statistics."""
     rows, vocab = logits.shape
     code = _lib.TYPE_CODES[logits.dtype]
     logprob = logits.new_empty(rows, dtype=torch.float32)
     entropy = torch.empty_like(logprob)
-    stats = logprob.new_empty((rows, 2))
     top_lp = logprob.new_empty((rows, top_k))
-    top_ids = logits.new_empty((rows, top_k), dtype=torch.int64)
-    if rows:
-        nbytes = _lib.workspace_bytes(logits, "tb_token_logprobs_workspace", rows, vocab, code,
-                                      top_k)
-        ws = logits.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-        _lib.call_on(logits, "tb_token_logprobs_fwd", logits.data_ptr(), code, _ld(logits),
-                     ids.data_ptr(), int(ids.dtype == torch.int64), temperature, top_k,
-                     logprob.data_ptr(), entropy.data_ptr(), top_lp.data_ptr(), top_ids.data_ptr(),
-                     stats.data_ptr(), rows, vocab, _lib.addr(ws), nbytes)
+    top_ids = logprob.new_empty((rows, top_k), dtype=torch.int64)
+    if not rows:
+        return logprob, entropy, top_lp, top_ids, logprob.new_empty(0)
+    # the workspace with the backward's statistics [rows, 3] behind it, as one allocation
+    nbytes = _lib.workspace_bytes(logits, "tb_token_logprobs_workspace", rows, vocab, code, top_k)
+    stats = logprob.new_empty(nbytes // 4 + 3 * rows)
+    at = stats.data_ptr()
+    _lib.call_on(logits, "tb_token_logprobs_fwd", logits.data_ptr(), code, _ld(logits),
+                 ids.data_ptr(), int(ids.dtype == torch.int64), temperature, top_k,
+                 logprob.data_ptr(), entropy.data_ptr(), top_lp.data_ptr(), top_ids.data_ptr(),
+                 at + nbytes, rows, vocab, at if nbytes else None, nbytes)
     return logprob, entropy, top_lp, top_ids, stats
 
 
@@ -64,7 +68,7 @@ class TokenLogprobsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, ids, top_k, temperature):
         logprob, entropy, top_lp, top_ids, stats = _forward(logits, ids, top_k, temperature)
-        ctx.save_for_backward(logits, ids, top_ids, stats, entropy)
+        ctx.save_for_backward(logits, ids, top_ids, stats)
         ctx.rest = (top_k, temperature)
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(top_ids)
@@ -73,7 +77,7 @@ class TokenLogprobsFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, g_lp, g_ent, g_top, _g_ids):
-        logits, ids, top_ids, stats, entropy = ctx.saved_tensors
+        logits, ids, top_ids, stats = ctx.saved_tensors
         top_k, temperature = ctx.rest
         if g_lp is None and g_ent is None and g_top is None:
             return None, None, None, None
@@ -84,9 +88,9 @@ class TokenLogprobsFn(torch.autograd.Function):
             _lib.call_on(logits, "tb_token_logprobs_bwd", logits.data_ptr(),
                          _lib.TYPE_CODES[logits.dtype], _ld(logits), ids.data_ptr(),
                          int(ids.dtype == torch.int64), temperature, top_k, top_ids.data_ptr(),
-                         stats.data_ptr(), entropy.data_ptr(), _lib.addr(g_lp), _lib.addr(g_ent),
-                         _lib.addr(g_top), grad.data_ptr(), grad.stride(0) if rows > 1 else vocab,
-                         rows, vocab)
+                         stats.data_ptr() + 4 * (stats.numel() - 3 * rows), _lib.addr(g_lp),
+                         _lib.addr(g_ent), _lib.addr(g_top), grad.data_ptr(),
+                         grad.stride(0) if rows > 1 else vocab, rows, vocab)
         return grad, None, None, None
 
 
@@ -112,10 +116,10 @@ def token_logprobs(logits, ids, top_k=0, temperature=1.0):
     temperature = float(temperature)
     if not 1e-4 <= temperature <= 1e4:
         raise ValueError(f"token_logprobs: temperature {temperature} outside [1e-4, 1e4]")
-    flat = logits.reshape(-1, vocab)
+    flat = logits if len(lead) == 1 else logits.reshape(-1, vocab)
     if flat.stride(1) != 1 or _ld(flat) < vocab:
         flat = flat.contiguous()
-    ids = ids.reshape(-1).contiguous()
+    ids = (ids if len(lead) == 1 else ids.reshape(-1)).contiguous()
     if _lib.needs_grad(flat):
         out = TokenLogprobsFn.apply(flat, ids, top_k, temperature)
     else:

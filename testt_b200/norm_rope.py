@@ -66,7 +66,8 @@ class NormRopeTokens(torch.autograd.Function):
         dkw = torch.empty_like(k_weight) if need[4] else None
         ws, nbytes = None, 0
         if need[3] or need[4]:
-            nbytes = _lib.workspace_bytes(qkv, "tb_norm_rope_bwd_workspace", rows, head_dim)
+            nbytes = _lib.workspace_bytes(qkv, "tb_norm_rope_bwd_workspace", rows, n_heads, n_kv,
+                                          head_dim)
             ws = cos.new_empty(max(nbytes // 4, 1))
         _lib.call_on(qkv, "tb_norm_rope_bwd", *(_lib.addr(g) for g in grads), qkv.data_ptr(), code,
                      _ld(qkv), _lib.addr(lora_q), _code(lora_q, code), _lib.addr(q_weight),
@@ -88,6 +89,14 @@ def _pair(a, b, dtype):
             None if b is None else b.to(torch.float32).contiguous())
 
 
+def _check(t, name, shape, index):
+    if t.shape != shape or t.get_device() != index:
+        raise ValueError(f"norm_rope_tokens: {name} {tuple(t.shape)} on {t.device}, expected "
+                         f"{shape} beside qkv")
+    if t.dtype not in _lib.TYPE_CODES:
+        raise TypeError(f"norm_rope_tokens: {name} must be fp16, bf16 or fp32, got {t.dtype}")
+
+
 def norm_rope_tokens(qkv, lora_q, lora_v, q_weight, k_weight, eps, cos, sin, pos_idx, batch, seq,
                      n_heads, n_kv, head_dim, weight_offset=0.0):
     """(q, k, v) token-major in qkv's dtype (fp16, bf16 or fp32), as rope.rope_tokens with each
@@ -98,42 +107,45 @@ def norm_rope_tokens(qkv, lora_q, lora_v, q_weight, k_weight, eps, cos, sin, pos
     views of wider rows. Differentiable in qkv, lora_q, lora_v, q_weight and k_weight."""
     _lib.require_cuda(qkv, lora_q, lora_v, q_weight, k_weight, cos, sin, pos_idx,
                       what="norm_rope_tokens")
-    if qkv.dtype not in _lib.TYPE_CODES:
-        raise TypeError(f"norm_rope_tokens: qkv must be fp16, bf16 or fp32, got {qkv.dtype}")
+    dtype, rows = qkv.dtype, qkv.shape[0] if qkv.dim() else 0
+    if dtype not in _lib.TYPE_CODES:
+        raise TypeError(f"norm_rope_tokens: qkv must be fp16, bf16 or fp32, got {dtype}")
     if n_heads <= 0 or n_kv < 0 or head_dim <= 0 or head_dim % 2:
         raise ValueError(f"norm_rope_tokens: {n_heads} / {n_kv} heads of {head_dim}")
-    if qkv.dim() != 2 or qkv.shape[1] != (n_heads + 2 * n_kv) * head_dim:
-        raise ValueError(f"norm_rope_tokens: qkv {tuple(qkv.shape)}, expected "
-                         f"[rows, {(n_heads + 2 * n_kv) * head_dim}]")
-    rows = qkv.shape[0]
-    for name, t, *shape in (("lora_q", lora_q, rows, n_heads * head_dim),
-                            ("lora_v", lora_v, rows, n_kv * head_dim),
-                            ("q_weight", q_weight, head_dim), ("k_weight", k_weight, head_dim)):
-        if t is not None:
-            if list(t.shape) != shape:
-                raise ValueError(f"norm_rope_tokens: {name} {tuple(t.shape)}, expected {shape}")
-            if t.dtype not in _lib.TYPE_CODES:
-                raise TypeError(f"norm_rope_tokens: {name} must be fp16, bf16 or fp32, got "
-                                f"{t.dtype}")
-    if pos_idx.dim() != 1 or pos_idx.shape[0] != rows:
-        raise ValueError(f"norm_rope_tokens: pos_idx {tuple(pos_idx.shape)}, expected {(rows,)}")
-    if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[0] < seq or cos.shape[1] % 2 or \
-            cos.shape[1] > head_dim:
+    width = (n_heads + 2 * n_kv) * head_dim
+    if qkv.dim() != 2 or qkv.shape[1] != width:
+        raise ValueError(f"norm_rope_tokens: qkv {tuple(qkv.shape)}, expected [rows, {width}]")
+    index = qkv.get_device()
+    if lora_q is not None:
+        _check(lora_q, "lora_q", (rows, n_heads * head_dim), index)
+    if lora_v is not None:
+        _check(lora_v, "lora_v", (rows, n_kv * head_dim), index)
+    if q_weight is not None:
+        _check(q_weight, "q_weight", (head_dim,), index)
+    if k_weight is not None:
+        _check(k_weight, "k_weight", (head_dim,), index)
+    rot = cos.shape[-1] if cos.dim() == 2 else -1
+    if rot < 0 or rot % 2 or rot > head_dim or cos.shape != sin.shape or cos.shape[0] < seq or \
+            cos.get_device() != index or sin.get_device() != index:
         raise ValueError(f"norm_rope_tokens: tables {tuple(cos.shape)} and {tuple(sin.shape)} for "
                          f"seq {seq}, head_dim {head_dim}")
-    if pos_idx.dtype not in (torch.int64, torch.int32):
-        raise TypeError(f"norm_rope_tokens: pos_idx must be int64 or int32, got {pos_idx.dtype}")
-    index = qkv.get_device()
-    for t in (lora_q, lora_v, q_weight, k_weight, cos, sin, pos_idx):
-        if t is not None and t.get_device() != index:
-            raise ValueError(f"norm_rope_tokens: operands on {t.device} and {qkv.device}")
-    if qkv.stride(1) != 1 or _ld(qkv) < qkv.shape[1]:
+    if pos_idx.dtype != torch.int64:
+        if pos_idx.dtype != torch.int32:
+            raise TypeError(f"norm_rope_tokens: pos_idx must be int64 or int32, got "
+                            f"{pos_idx.dtype}")
+        pos_idx = pos_idx.to(torch.int64)
+    if pos_idx.dim() != 1 or pos_idx.shape[0] != rows or pos_idx.get_device() != index:
+        raise ValueError(f"norm_rope_tokens: pos_idx {tuple(pos_idx.shape)} on {pos_idx.device}, "
+                         f"expected {(rows,)} on {qkv.device}")
+    if qkv.stride(1) != 1 or _ld(qkv) < width:
         qkv = qkv.contiguous()
-    lora_q, lora_v = _pair(lora_q, lora_v, qkv.dtype)
-    q_weight, k_weight = _pair(q_weight, k_weight, qkv.dtype)
-    args = (qkv, lora_q, lora_v, q_weight, k_weight, float(eps),
-            cos.to(torch.float32).contiguous(), sin.to(torch.float32).contiguous(),
-            pos_idx.to(torch.int64).contiguous(), int(batch), int(seq), int(n_heads), int(n_kv),
+    if lora_q is not None or lora_v is not None:
+        lora_q, lora_v = _pair(lora_q, lora_v, dtype)
+    q_weight, k_weight = _pair(q_weight, k_weight, dtype)
+    if cos.dtype != torch.float32 or sin.dtype != torch.float32:
+        cos, sin = cos.to(torch.float32), sin.to(torch.float32)
+    args = (qkv, lora_q, lora_v, q_weight, k_weight, float(eps), cos.contiguous(),
+            sin.contiguous(), pos_idx.contiguous(), int(batch), int(seq), int(n_heads), int(n_kv),
             int(head_dim), float(weight_offset))
     if _lib.needs_grad(qkv, lora_q, lora_v, q_weight, k_weight):
         return NormRopeTokens.apply(*args)
