@@ -92,6 +92,46 @@ __device__ __forceinline__ void store8(void *p, int64_t i, const float (&f)[8]) 
   }
 }
 
+// Two fp32 values in one 64-bit register pair: sm_100's packed fp32 instructions do two multiply-adds
+// in one issue slot (each rounded as the scalar one).
+struct F2 {
+  uint64_t v;
+};
+
+__device__ __forceinline__ F2 make_f2(float lo, float hi) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+  return r;
+}
+
+__device__ __forceinline__ F2 both(float x) { return make_f2(x, x); }
+
+__device__ __forceinline__ float2 parts(F2 a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+  return r;
+}
+
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+
+__device__ __forceinline__ F2 neg2(F2 a) { return F2{a.v ^ 0x8000000080000000ull}; }
+
 // Runs the statement with the constant `T` bound to the element type `t` (already checked).
 #define TB_WITH_TYPE(t, T, ...)                                 \
   do {                                                          \

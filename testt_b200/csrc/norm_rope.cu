@@ -6,12 +6,20 @@
 //   dn = the transposed rotation of dy     g = dn (w0 + w)     dx = r (g - x r^2 mean(g x))
 //   dw = sum over tokens and heads of dn x r
 // x is read again and both means come out of one set of shuffles, so the forward stores nothing
-// for the backward. dw: each CTA walks tokens blockIdx, + gridDim, ... and keeps its sums in
-// registers; a second kernel adds the CTAs' sums in order, so results do not depend on timing.
+// for the backward. dw: each lane keeps its sums over its warp's tokens; they are added in order of
+// the lanes, then (a second kernel) of the CTAs, so results do not depend on timing.
+//
+// 16411 tokens of 32 + 8 + 8 heads of 128, half of each turned, bf16: forward 82 us (403 MB, 4.9
+// TB/s), backward 135 + 3 us (571 MB, 4.2 TB/s); a plain copy runs at 6.55 TB/s. Bound by issue and
+// shared-memory reads at 16 to 24 warps an SM, not by DRAM: one CTA a token with everything in
+// registers took 259 / 291 us (one CTA an SM), deeper rings change nothing. Packed fp32 pairs halve
+// the arithmetic's issue slots; the rotation's factors lie in shared memory once a warp and token,
+// as 32 registers less a lane allow half as many warps again.
 //
 // Beside tb_rope_tokens_* (solution/rope.py:24-176), which has no norm; positions and tables as
 // there. The reference's model has no head norms.
 #include <initializer_list>
+#include <type_traits>
 
 #include "dtypes.cuh"
 
@@ -20,6 +28,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
+constexpr int kFwdPerSm = 3, kBwdPerSm = 2;  // resident CTAs of the vector kernels
 constexpr uint32_t kAll = 0xffffffffu;
 
 struct NormDims {
@@ -28,65 +37,78 @@ struct NormDims {
   float eps, w0, inv_d;
 };
 
-// Four neighbouring values as loaded: 8 bytes of a 16-bit type, 16 of fp32.
-template <int T>
-struct Quad {
-  using type = uint2;
-  static __device__ __forceinline__ void get(const type &v, float (&f)[4]) {
-    const float2 a = Elem<T>::get2(v.x), b = Elem<T>::get2(v.y);
-    f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
+// V neighbouring values as loaded (16 bytes, or 8 for four 16-bit values) and as fp32 pairs.
+template <int T, int V>
+struct Vec {
+  using type = typename std::conditional<V == 8, uint4, uint2>::type;
+  static __device__ __forceinline__ void get(const type &v, F2 (&f)[V / 2]) {
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(&v);
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      const float2 a = Elem<T>::get2(w[i]);
+      f[i] = make_f2(a.x, a.y);
+    }
   }
-  static __device__ __forceinline__ type put(const float (&f)[4]) {
-    return make_uint2(Elem<T>::put2(f[0], f[1]), Elem<T>::put2(f[2], f[3]));
+  static __device__ __forceinline__ type put(const F2 (&f)[V / 2]) {
+    type v;
+    uint32_t *w = reinterpret_cast<uint32_t *>(&v);
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      const float2 a = parts(f[i]);
+      w[i] = Elem<T>::put2(a.x, a.y);
+    }
+    return v;
   }
-  static __device__ __forceinline__ type zero() { return make_uint2(0, 0); }
 };
 
-template <>
-struct Quad<TB_FP32> {
-  using type = float4;
-  static __device__ __forceinline__ void get(const type &v, float (&f)[4]) {
-    f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+template <int V>
+struct Vec<TB_FP32, V> {
+  struct type {
+    float4 q[V / 4];
+  };
+  static __device__ __forceinline__ void get(const type &v, F2 (&f)[V / 2]) {
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i) {
+      f[2 * i] = make_f2(v.q[i].x, v.q[i].y);
+      f[2 * i + 1] = make_f2(v.q[i].z, v.q[i].w);
+    }
   }
-  static __device__ __forceinline__ type put(const float (&f)[4]) {
-    return make_float4(f[0], f[1], f[2], f[3]);
+  static __device__ __forceinline__ type put(const F2 (&f)[V / 2]) {
+    type v;
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i) {
+      const float2 a = parts(f[2 * i]), b = parts(f[2 * i + 1]);
+      v.q[i] = make_float4(a.x, a.y, b.x, b.y);
+    }
+    return v;
   }
-  static __device__ __forceinline__ type zero() { return make_float4(0.f, 0.f, 0.f, 0.f); }
 };
 
-template <int T>
-__device__ __forceinline__ typename Quad<T>::type load4(const void *p, int64_t i) {
-  return __ldg(reinterpret_cast<const typename Quad<T>::type *>(
-      static_cast<const typename Elem<T>::type *>(p) + i));
+template <int T, int V>
+__device__ __forceinline__ typename Vec<T, V>::type load_raw(const void *p, int64_t i) {
+  const typename Elem<T>::type *q = static_cast<const typename Elem<T>::type *>(p) + i;
+  if constexpr (T == TB_FP32) {
+    typename Vec<T, V>::type v;
+#pragma unroll
+    for (int j = 0; j < V / 4; ++j) v.q[j] = __ldg(reinterpret_cast<const float4 *>(q) + j);
+    return v;
+  } else {
+    return __ldg(reinterpret_cast<const typename Vec<T, V>::type *>(q));
+  }
 }
 
-template <int T>
-__device__ __forceinline__ void store4(void *p, int64_t i, const float (&f)[4]) {
-  *reinterpret_cast<typename Quad<T>::type *>(static_cast<typename Elem<T>::type *>(p) + i) =
-      Quad<T>::put(f);
+template <int V>
+__device__ __forceinline__ void fill(F2 (&f)[V], float v) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) f[i] = both(v);
 }
 
 // Sum over groups of `lanes` (a power of two) neighbouring lanes; every lane gets the total.
 __device__ __forceinline__ float group_sum(float v, int lanes) {
-  for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    if (o < lanes) v += __shfl_xor_sync(kAll, v, o);
   return v;
-}
-
-// The two quads of a lane: lanes below rot / 8 hold a rotation's pair (four dims of each half),
-// the others two neighbouring quads of the rest.
-struct Chunks {
-  int a, b;
-  bool live, turn;
-};
-
-__device__ __forceinline__ Chunks chunks_of(int lane, int d, int rot) {
-  const int pairs = rot / 8;
-  Chunks c;
-  c.turn = lane < pairs;
-  c.a = c.turn ? lane * 4 : rot + (lane - pairs) * 8;
-  c.b = c.turn ? rot / 2 + lane * 4 : c.a + 4;
-  c.live = lane < d / 8;
-  return c;
 }
 
 // Output (or gradient) row of head row hr: q [rows, nh, d], k and v [rows, nkv, d].
@@ -102,251 +124,480 @@ __device__ __forceinline__ P pick(P q, P k, P v, const NormDims &dm, int64_t tok
   return key ? k : v;
 }
 
-template <int T>
-__device__ __forceinline__ void load_weight(const void *w, float w0, int i, float (&f)[4]) {
-  if (w == nullptr) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) f[e] = 1.f;
-  } else {
-    Quad<T>::get(load4<T>(w, i), f);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) f[e] += w0;
-  }
-}
+// How the vector kernels spread head rows: `lanes` lanes to a head row, each with two chunks of V
+// dims (lanes below rot / 2V a rotation's pair, one chunk of each half; the others two neighbouring
+// chunks of the rest), 32 / lanes head rows of one kind (q, k or v) to a group, a group to a warp
+// at a time. `parts` warps share a token's groups (one, when there are many tokens).
+struct Spread {
+  int lanes, at_once, gq, gk, groups, parts;  // groups of q, of k (and of v), all of them
+};
 
-template <int L>
-__device__ __forceinline__ void add4(const void *p, int64_t i, float (&f)[4]) {
-  float a[4];
-  Quad<L>::get(load4<L>(p, i), a);
-#pragma unroll
-  for (int e = 0; e < 4; ++e) f[e] += a[e];
-}
-
-// The rotation's factors of a token at a lane's quads.
-struct Turn {
-  float c1[4], c2[4], s1[4], s2[4];
-  __device__ __forceinline__ void load(const float *cosv, const float *sinv, int64_t row, int rot,
-                                       const Chunks &ch) {
-    Quad<TB_FP32>::get(load4<TB_FP32>(cosv, row * rot + ch.a), c1);
-    Quad<TB_FP32>::get(load4<TB_FP32>(cosv, row * rot + ch.b), c2);
-    Quad<TB_FP32>::get(load4<TB_FP32>(sinv, row * rot + ch.a), s1);
-    Quad<TB_FP32>::get(load4<TB_FP32>(sinv, row * rot + ch.b), s2);
+template <int V>
+struct Lane {
+  int a, b, slot;  // first dims of the two chunks; the head row in the group
+  bool live, turn;
+  __device__ __forceinline__ Lane(const NormDims &dm, const Spread &sp) {
+    const int lane = threadIdx.x & (sp.lanes - 1), pairs = dm.rot / (2 * V);
+    slot = (threadIdx.x & 31) / sp.lanes;
+    turn = lane < pairs;
+    a = turn ? lane * V : dm.rot + (lane - pairs) * 2 * V;
+    b = turn ? dm.rot / 2 + lane * V : a + V;
+    live = lane < dm.d / (2 * V);
   }
 };
 
-// `lanes` lanes per head row, so 32 / lanes head rows at a time to a warp. A warp takes a token
-// and every `parts`-th such group of its head rows, two groups in flight; the rotation's factors
-// are loaded once for them. W: the weights' type, L: the LoRA rows'.
-template <int T, int L, int W>
-__global__ void __launch_bounds__(kThreads, 4)
+// w0 + weight of q and of k in fp32, in shared memory ([2][d]); 1 without a weight.
+template <int W>
+__device__ __forceinline__ void stage_weights(float *ws, const void *qw, const void *kw, float w0,
+                                              int d) {
+  for (int i = threadIdx.x; i < 2 * d; i += kThreads) {
+    const void *w = i < d ? qw : kw;
+    ws[i] = w == nullptr ? 1.f : w0 + load1<W>(w, i < d ? i : i - d);
+  }
+}
+
+// ---- the walk of the vector kernels ----------------------------------------------------------
+// The rows of the next stages - 1 groups of a warp's walk are on their way into the lane's own slots
+// of shared memory (cp.async: no registers held, and no barrier, since a lane reads only what it
+// copied).
+
+constexpr int kFwdStages = 3, kBwdStages = 3;
+
+template <int B>
+__device__ __forceinline__ void copy_async(void *dst, const void *src) {
+  if constexpr (B == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src)
+                 : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(dst)), "l"(src),
+                 "n"(B)
+                 : "memory");
+}
+
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// A warp's walk: groups part, part + parts, ... of tokens tok, + stride, ...
+struct Walk {
+  int part;
+  int64_t tok, stride;
+  __device__ __forceinline__ Walk(const NormDims &dm, const Spread &sp) {
+    const int wid = blockIdx.x * kWarps + (threadIdx.x >> 5);
+    part = wid % sp.parts;
+    stride = (int)gridDim.x * kWarps / sp.parts;
+    tok = wid / sp.parts < stride ? wid / sp.parts : dm.rows;  // leftover warps do nothing
+  }
+};
+
+// Where the walk's copies are, stages - 1 groups ahead of the work: the lane's place in the qkv row
+// and in the kind's gradient or LoRA-shaped rows, moved on by constants within a kind.
+struct Ahead {
+  int64_t tok;
+  int g, end, left;  // group, first of the next kind, head rows from the lane's to the kind's end
+  int kind;
+  const char *x, *y;
+
+  // bases: of q-, k- and v-shaped rows (may be NULL); es: bytes of an element
+  __device__ __forceinline__ void locate(const NormDims &dm, const Spread &sp, const Walk &wk,
+                                         int slot, const char *qkv, const char *bq,
+                                         const char *bk, const char *bv, int es) {
+    if (g >= sp.groups) {
+      g = wk.part;
+      tok += wk.stride;
+    }
+    kind = g < sp.gq ? 0 : g < sp.gq + sp.gk ? 1 : 2;
+    const int start = kind == 0 ? 0 : kind == 1 ? sp.gq : sp.gq + sp.gk;
+    end = kind == 0 ? sp.gq : kind == 1 ? sp.gq + sp.gk : sp.groups;
+    const int n = kind == 0 ? dm.nh : dm.nkv, head = (g - start) * sp.at_once + slot;
+    const int first = kind == 0 ? 0 : kind == 1 ? dm.nh : dm.nh + dm.nkv;
+    left = tok < dm.rows ? n - head : 0;
+    x = qkv + (tok * dm.ld + (first + head) * dm.d) * es;
+    y = kind == 0 ? bq : kind == 1 ? bk : bv;
+    if (y != nullptr) y += (tok * n + head) * (int64_t)dm.d * es;
+  }
+  __device__ __forceinline__ bool next(const Spread &sp, int step, int bytes) {
+    g += sp.parts;
+    left -= step;
+    x += bytes;
+    y += bytes;
+    return g < end;
+  }
+};
+
+// A warp's table of a token's rotation in shared memory, four rows of fp32 quads laid out [row][quad]
+// [lane]: all its head rows use the same factors, so a lane reads them where it needs them instead
+// of holding 4 V registers. Forward rows: y1 = r (x1 A + x2 B), y2 = r (x2 C + x1 D) with the
+// weights inside (A = w1 c1, B = -w2 s1, C = w2 c2, D = w1 s2); backward rows: c1, -s1, c2, s2.
+// Lanes past rot turn by cosine 1, sine 0. The head rows' lanes share the work.
+template <int V, bool kWeights>
+__device__ __forceinline__ void make_table(float4 *tab, const float *cosv, const float *sinv,
+                                           int64_t row, const float *w, const Lane<V> &ln,
+                                           const Spread &sp) {
+  const int lane = threadIdx.x & (sp.lanes - 1);
+  __syncwarp();
+  for (int i = ln.slot; i < V / 4 && ln.live; i += sp.at_once) {
+    float4 c1 = make_float4(1.f, 1.f, 1.f, 1.f), c2 = c1;
+    float4 s1 = make_float4(0.f, 0.f, 0.f, 0.f), s2 = s1;
+    if (ln.turn) {
+      c1 = __ldg(reinterpret_cast<const float4 *>(cosv + row + ln.a) + i);
+      c2 = __ldg(reinterpret_cast<const float4 *>(cosv + row + ln.b) + i);
+      s1 = __ldg(reinterpret_cast<const float4 *>(sinv + row + ln.a) + i);
+      s2 = __ldg(reinterpret_cast<const float4 *>(sinv + row + ln.b) + i);
+    }
+    float4 w1 = make_float4(1.f, 1.f, 1.f, 1.f), w2 = w1;
+    if (kWeights) {
+      w1 = reinterpret_cast<const float4 *>(w + ln.a)[i];
+      w2 = reinterpret_cast<const float4 *>(w + ln.b)[i];
+    }
+    float4 *t = tab + i * sp.lanes + lane;
+    const int next = (V / 4) * sp.lanes;
+    t[0] = make_float4(w1.x * c1.x, w1.y * c1.y, w1.z * c1.z, w1.w * c1.w);
+    const float4 m = kWeights ? w2 : w1;
+    t[next] = make_float4(-m.x * s1.x, -m.y * s1.y, -m.z * s1.z, -m.w * s1.w);
+    t[2 * next] = make_float4(w2.x * c2.x, w2.y * c2.y, w2.z * c2.z, w2.w * c2.w);
+    t[3 * next] = make_float4(w1.x * s2.x, w1.y * s2.y, w1.z * s2.z, w1.w * s2.w);
+  }
+  __syncwarp();
+}
+
+struct Quad2 {
+  F2 lo, hi;
+};
+
+__device__ __forceinline__ Quad2 quad_at(const float4 *p) {
+  const float4 q = *p;
+  return Quad2{make_f2(q.x, q.y), make_f2(q.z, q.w)};
+}
+
+template <int V>
+__device__ __forceinline__ float square_sum(const F2 (&x1)[V], const F2 (&x2)[V]) {
+  F2 s = both(0.f), t = s;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    s = fma2(x1[i], x1[i], s);
+    t = fma2(x2[i], x2[i], t);
+  }
+  const float2 p = parts(add2(s, t));
+  return p.x + p.y;
+}
+
+// W: the weights' type, L: the LoRA rows'. The weights are folded into a token's factors, so that a
+// pair costs four multiply-adds and two products with r.
+template <int T, int V, int L, int W>
+__global__ void __launch_bounds__(kThreads, kFwdPerSm)
     norm_rope_fwd(const void *__restrict__ qkv, const void *__restrict__ lq,
                   const void *__restrict__ lv, const void *__restrict__ qw,
                   const void *__restrict__ kw, const float *__restrict__ cosv,
                   const float *__restrict__ sinv, const int64_t *__restrict__ pos_idx, void *q,
-                  void *k, void *v, NormDims dm, FastDiv seq_div, FastDiv parts, int lanes) {
+                  void *k, void *v, NormDims dm, Spread sp, FastDiv seq_div) {
   pdl_wait();
   pdl_release();
-  constexpr int kGroups = 2;
-  const uint32_t unit = blockIdx.x * kWarps + (threadIdx.x >> 5);
-  uint32_t tok32, part;
-  parts.divmod(unit, tok32, part);
-  const int64_t tok = tok32;
-  if (tok >= dm.rows) return;
-  const int lane = threadIdx.x & (lanes - 1), slot = (threadIdx.x & 31) / lanes;
-  const int rows_at_once = 32 / lanes, total = dm.nh + 2 * dm.nkv;
-  const Chunks ch = chunks_of(lane, dm.d, dm.rot);
-  const int64_t pos = __ldg(pos_idx + tok);
-  const bool inside = pos >= 0 && pos < dm.slots;
-  Turn t;
-  bool turned = false;
-  for (int hr0 = part * rows_at_once; hr0 < total; hr0 += kGroups * (int)parts.d * rows_at_once) {
-    float x1[kGroups][4], x2[kGroups][4], r[kGroups];
-    typename Quad<T>::type r1[kGroups], r2[kGroups];
-    int hr[kGroups];
-#pragma unroll
-    for (int j = 0; j < kGroups; ++j) {
-      hr[j] = hr0 + j * (int)parts.d * rows_at_once + slot;
-      r1[j] = r2[j] = Quad<T>::zero();
-      if (ch.live && hr[j] < total && inside) {
-        const int64_t at = tok * dm.ld + (int64_t)hr[j] * dm.d;
-        r1[j] = load4<T>(qkv, at + ch.a);
-        r2[j] = load4<T>(qkv, at + ch.b);
-      }
+  using Raw = typename Vec<T, V>::type;
+  constexpr int kB = V * elem_size<T>(), es = elem_size<T>();
+  extern __shared__ uint4 shared[];
+  Raw(*ring)[2][kThreads] = reinterpret_cast<Raw(*)[2][kThreads]>(shared);
+  float *ws = reinterpret_cast<float *>(ring + kFwdStages);
+  float4 *tab = reinterpret_cast<float4 *>(ws + 2 * dm.d) + (threadIdx.x >> 5) * V * sp.lanes;
+  const float4 *mine = tab + (threadIdx.x & (sp.lanes - 1));
+  const Lane<V> ln(dm, sp);
+  const Walk wk(dm, sp);
+  const int step = sp.parts * sp.at_once, bytes = step * dm.d * es;
+  Ahead ahead;
+  ahead.tok = wk.tok;
+  ahead.g = wk.part;
+  auto locate = [&]() {
+    ahead.locate(dm, sp, wk, ln.slot, static_cast<const char *>(qkv), nullptr, nullptr, nullptr, es);
+  };
+  locate();
+  auto fetch = [&](int stage) {
+    if (ln.live && ahead.left > 0) {
+      copy_async<kB>(&ring[stage][0][threadIdx.x], ahead.x + ln.a * es);
+      copy_async<kB>(&ring[stage][1][threadIdx.x], ahead.x + ln.b * es);
     }
-    if (!turned && ch.live && ch.turn && inside) {
-      uint32_t b32, t32;
-      seq_div.divmod((uint32_t)pos, b32, t32);
-      t.load(cosv, sinv, t32, dm.rot, ch);
-      turned = true;
-    }
+    copies_commit();
+    if (!ahead.next(sp, step, bytes)) locate();
+  };
+  int64_t pos = wk.tok < dm.rows ? __ldg(pos_idx + wk.tok) : -1;
 #pragma unroll
-    for (int j = 0; j < kGroups; ++j) {
-      Quad<T>::get(r1[j], x1[j]);
-      Quad<T>::get(r2[j], x2[j]);
-      const bool isq = hr[j] < dm.nh, isv = hr[j] >= dm.nh + dm.nkv && hr[j] < total;
-      const void *l = isq ? lq : isv ? lv : nullptr;
-      if (l != nullptr && ch.live && inside) {
-        const int64_t li = isq ? (tok * dm.nh + hr[j]) * (int64_t)dm.d
-                               : (tok * dm.nkv + hr[j] - dm.nh - dm.nkv) * (int64_t)dm.d;
-        add4<L>(l, li + ch.a, x1[j]);
-        add4<L>(l, li + ch.b, x2[j]);
-      }
-      float ss = 0.f;
+  for (int i = 0; i < kFwdStages - 1; ++i) fetch(i);
+  stage_weights<W>(ws, qw, kw, dm.w0, dm.d);
+  __syncthreads();
+  int stage = 0;
+  for (int64_t tok = wk.tok; tok < dm.rows; tok += wk.stride) {
+    const bool inside = pos >= 0 && pos < dm.slots;
+    uint32_t b32, t32 = 0;
+    if (inside) seq_div.divmod((uint32_t)pos, b32, t32);
+    if (tok + wk.stride < dm.rows) pos = __ldg(pos_idx + tok + wk.stride);
+    int g = wk.part;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) ss += x1[j][e] * x1[j][e] + x2[j][e] * x2[j][e];
-      r[j] = rsqrtf(group_sum(ss, lanes) * dm.inv_d + dm.eps);
-    }
-#pragma unroll
-    for (int j = 0; j < kGroups; ++j) {
-      if (!ch.live || hr[j] >= total) continue;
-      if (hr[j] < dm.nh + dm.nkv && inside) {
-        const void *w = hr[j] < dm.nh ? qw : kw;
-        float w1[4], w2[4];
-        load_weight<W>(w, dm.w0, ch.a, w1);
-        load_weight<W>(w, dm.w0, ch.b, w2);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float n1 = x1[j][e] * r[j] * w1[e], n2 = x2[j][e] * r[j] * w2[e];
-          x1[j][e] = ch.turn ? n1 * t.c1[e] - n2 * t.s1[e] : n1;
-          x2[j][e] = ch.turn ? n2 * t.c2[e] + n1 * t.s2[e] : n2;
+    for (int kind = 0; kind < 3; ++kind) {
+      const int g0 = kind == 0 ? 0 : kind == 1 ? sp.gq : sp.gq + sp.gk;
+      const int g1 = kind == 0 ? sp.gq : kind == 1 ? sp.gq + sp.gk : sp.groups;
+      if (g >= g1) continue;
+      const int n = kind == 0 ? dm.nh : dm.nkv;
+      if (kind < 2)
+        make_table<V, true>(tab, cosv, sinv, (int64_t)t32 * dm.rot, ws + kind * dm.d, ln, sp);
+      int left = n - (g - g0) * sp.at_once - ln.slot;
+      const int64_t at = (tok * n + (n - left)) * (int64_t)dm.d;
+      char *out = static_cast<char *>(kind == 0 ? q : kind == 1 ? k : v) + at * es;
+      const void *l = kind == 0 ? lq : kind == 1 ? nullptr : lv;
+      const char *lora = static_cast<const char *>(l) + at * elem_size<L>();
+      for (; g < g1; g += sp.parts) {
+        const bool live = ln.live && left > 0;
+        typename Vec<L, V>::type l1, l2;
+        if (kind != 1 && l != nullptr && live) {
+          l1 = load_raw<L, V>(lora, ln.a);
+          l2 = load_raw<L, V>(lora, ln.b);
         }
+        copies_wait<kFwdStages - 2>();
+        F2 x1[V / 2], x2[V / 2];
+        if (live && inside) {
+          Vec<T, V>::get(ring[stage][0][threadIdx.x], x1);
+          Vec<T, V>::get(ring[stage][1][threadIdx.x], x2);
+          if (kind != 1 && l != nullptr) {
+            F2 y1[V / 2], y2[V / 2];
+            Vec<L, V>::get(l1, y1);
+            Vec<L, V>::get(l2, y2);
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) {
+              x1[i] = add2(x1[i], y1[i]);
+              x2[i] = add2(x2[i], y2[i]);
+            }
+          }
+        } else {
+          fill(x1, 0.f);
+          fill(x2, 0.f);
+        }
+        fetch((stage + kFwdStages - 1) % kFwdStages);
+        stage = (stage + 1) % kFwdStages;
+        if (kind < 2) {
+          const float ss = group_sum(square_sum(x1, x2), sp.lanes);
+          const F2 r = both(rsqrtf(fmaf(ss, dm.inv_d, dm.eps)));
+          if (live && inside) {
+            const int next = (V / 4) * sp.lanes;
+#pragma unroll
+            for (int i = 0; i < V / 4; ++i) {
+              const float4 *p = mine + i * sp.lanes;
+              const Quad2 A = quad_at(p), B = quad_at(p + next), C = quad_at(p + 2 * next),
+                          D = quad_at(p + 3 * next);
+              const F2 y = fma2(x1[2 * i], A.lo, mul2(x2[2 * i], B.lo));
+              const F2 z = fma2(x1[2 * i + 1], A.hi, mul2(x2[2 * i + 1], B.hi));
+              x2[2 * i] = mul2(r, fma2(x2[2 * i], C.lo, mul2(x1[2 * i], D.lo)));
+              x2[2 * i + 1] = mul2(r, fma2(x2[2 * i + 1], C.hi, mul2(x1[2 * i + 1], D.hi)));
+              x1[2 * i] = mul2(r, y);
+              x1[2 * i + 1] = mul2(r, z);
+            }
+          }
+        }
+        if (live) {
+          *reinterpret_cast<Raw *>(out + ln.a * es) = Vec<T, V>::put(x1);
+          *reinterpret_cast<Raw *>(out + ln.b * es) = Vec<T, V>::put(x2);
+        }
+        left -= step;
+        out += bytes;
+        lora += (int64_t)step * dm.d * elem_size<L>();
       }
-      int64_t at;
-      void *dst = pick(q, k, v, dm, tok, hr[j], at);
-      store4<T>(dst, at + ch.a, x1[j]);
-      store4<T>(dst, at + ch.b, x2[j]);
     }
   }
+  copies_wait<0>();
 }
 
-// Backward. Each warp keeps one group of head rows and walks tokens warp / groups, + stride, ...,
-// the next token's rows in flight while this one's are worked on; so a lane's head row, weights
-// and weight sums stay the same. part (may be NULL): fp32 [gridDim, 2, d], this CTA's sums of dqw
-// and dkw.
-template <int T, int L, int W>
-__global__ void __launch_bounds__(kThreads, 3)
+// Backward. A lane's weight sums of the kind at hand are in registers, those of the walk in its own
+// place of shared memory. part (may be NULL): fp32 [gridDim, 2, d], this CTA's sums of dqw and dkw.
+template <int T, int V, int L, int W>
+__global__ void __launch_bounds__(kThreads, kBwdPerSm)
     norm_rope_bwd(const void *__restrict__ dq, const void *__restrict__ dk,
                   const void *__restrict__ dv, const void *__restrict__ qkv,
                   const void *__restrict__ lq, const void *__restrict__ qw,
                   const void *__restrict__ kw, const float *__restrict__ cosv,
                   const float *__restrict__ sinv, const int64_t *__restrict__ pos_idx,
-                  void *__restrict__ dqkv, float *__restrict__ part, NormDims dm, FastDiv seq_div,
-                  int lanes, int groups) {
+                  void *__restrict__ dqkv, float *__restrict__ part, NormDims dm, Spread sp,
+                  FastDiv seq_div) {
   pdl_wait();
   pdl_release();
-  using Raw = typename Quad<T>::type;
-  const int wid = blockIdx.x * kWarps + (threadIdx.x >> 5);
-  const int stride = (int)gridDim.x * kWarps / groups;  // tokens between a warp's
-  const int lane = threadIdx.x & (lanes - 1), slot = (threadIdx.x & 31) / lanes;
-  const int rows_at_once = 32 / lanes, total = dm.nh + 2 * dm.nkv;
-  const int hr = (wid % groups) * rows_at_once + slot;
-  const Chunks ch = chunks_of(lane, dm.d, dm.rot);
-  const bool live = ch.live && hr < total, normed = live && hr < dm.nh + dm.nkv;
-  const int64_t width = (int64_t)total * dm.d;
-  float a1[4] = {0.f, 0.f, 0.f, 0.f}, a2[4] = {0.f, 0.f, 0.f, 0.f};
-  float w1[4], w2[4];
-  if (normed) {
-    load_weight<W>(hr < dm.nh ? qw : kw, dm.w0, ch.a, w1);
-    load_weight<W>(hr < dm.nh ? qw : kw, dm.w0, ch.b, w2);
-  }
-  int64_t tok = wid / groups < stride ? wid / groups : dm.rows;  // warps left over do nothing
-  Raw g1 = Quad<T>::zero(), g2 = g1, x1 = g1, x2 = g1;
-  int64_t pos = -1;
-  auto load = [&](int64_t at_tok) {
-    g1 = g2 = x1 = x2 = Quad<T>::zero();
-    if (at_tok < dm.rows) {
-      pos = __ldg(pos_idx + at_tok);
-      if (live) {
-        int64_t at;
-        const void *src = pick(dq, dk, dv, dm, at_tok, hr, at);
-        if (src != nullptr) {
-          g1 = load4<T>(src, at + ch.a);
-          g2 = load4<T>(src, at + ch.b);
-        }
-      }
-      if (normed) {
-        const int64_t at = at_tok * dm.ld + (int64_t)hr * dm.d;
-        x1 = load4<T>(qkv, at + ch.a);
-        x2 = load4<T>(qkv, at + ch.b);
-      }
-    }
+  using Raw = typename Vec<T, V>::type;
+  constexpr int kB = V * elem_size<T>(), es = elem_size<T>();
+  extern __shared__ uint4 shared[];
+  Raw(*ring)[4][kThreads] = reinterpret_cast<Raw(*)[4][kThreads]>(shared);
+  F2(*sums)[V][kThreads] = reinterpret_cast<F2(*)[V][kThreads]>(ring + kBwdStages);
+  float *ws = reinterpret_cast<float *>(sums + 2);
+  float4 *tab = reinterpret_cast<float4 *>(ws + 2 * dm.d) + (threadIdx.x >> 5) * V * sp.lanes;
+  const float4 *mine = tab + (threadIdx.x & (sp.lanes - 1));
+  const Lane<V> ln(dm, sp);
+  const Walk wk(dm, sp);
+  const int total = dm.nh + 2 * dm.nkv;
+  const int step = sp.parts * sp.at_once, bytes = step * dm.d * es;
+#pragma unroll
+  for (int i = 0; i < V; ++i) sums[0][i][threadIdx.x] = sums[1][i][threadIdx.x] = both(0.f);
+  Ahead ahead;
+  ahead.tok = wk.tok;
+  ahead.g = wk.part;
+  auto locate = [&]() {
+    ahead.locate(dm, sp, wk, ln.slot, static_cast<const char *>(qkv),
+                 static_cast<const char *>(dq), static_cast<const char *>(dk),
+                 static_cast<const char *>(dv), es);
   };
-  load(tok);
-  for (; tok < dm.rows; tok += stride) {
+  locate();
+  const bool has[3] = {dq != nullptr, dk != nullptr, dv != nullptr};
+  auto fetch = [&](int stage) {
+    if (ln.live && ahead.left > 0) {
+      if (ahead.kind == 0 ? has[0] : ahead.kind == 1 ? has[1] : has[2]) {
+        copy_async<kB>(&ring[stage][0][threadIdx.x], ahead.y + ln.a * es);
+        copy_async<kB>(&ring[stage][1][threadIdx.x], ahead.y + ln.b * es);
+      }
+      if (ahead.kind < 2) {
+        copy_async<kB>(&ring[stage][2][threadIdx.x], ahead.x + ln.a * es);
+        copy_async<kB>(&ring[stage][3][threadIdx.x], ahead.x + ln.b * es);
+      }
+    }
+    copies_commit();
+    if (!ahead.next(sp, step, bytes)) locate();
+  };
+  int64_t pos = wk.tok < dm.rows ? __ldg(pos_idx + wk.tok) : -1;
+#pragma unroll
+  for (int i = 0; i < kBwdStages - 1; ++i) fetch(i);
+  stage_weights<W>(ws, qw, kw, dm.w0, dm.d);
+  __syncthreads();
+  int stage = 0;
+  for (int64_t tok = wk.tok; tok < dm.rows; tok += wk.stride) {
     const bool inside = pos >= 0 && pos < dm.slots;
-    uint32_t b32 = 0, t32 = 0;
+    uint32_t b32, t32 = 0;
     if (inside) seq_div.divmod((uint32_t)pos, b32, t32);
-    Turn t;
-    if (normed && ch.turn) t.load(cosv, sinv, t32, dm.rot, ch);
-    float f1[4], f2[4], y1[4], y2[4];
-    Quad<T>::get(g1, f1);
-    Quad<T>::get(g2, f2);
-    Quad<T>::get(x1, y1);
-    Quad<T>::get(x2, y2);
-    if (lq != nullptr && live && hr < dm.nh) {
-      const int64_t li = (tok * dm.nh + hr) * (int64_t)dm.d;
-      add4<L>(lq, li + ch.a, y1);
-      add4<L>(lq, li + ch.b, y2);
-    }
-    load(tok + stride);
-    float ss = 0.f, gx = 0.f;
-    if (normed) {
+    make_table<V, false>(tab, cosv, sinv, (int64_t)t32 * dm.rot, nullptr, ln, sp);
+    if (tok + wk.stride < dm.rows) pos = __ldg(pos_idx + tok + wk.stride);
+    int g = wk.part;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (ch.turn) {
-          const float d1 = f1[e] * t.c1[e] + f2[e] * t.s2[e];
-          const float d2 = f2[e] * t.c2[e] - f1[e] * t.s1[e];
-          f1[e] = d1;
-          f2[e] = d2;
+    for (int kind = 0; kind < 3; ++kind) {
+      const int g0 = kind == 0 ? 0 : kind == 1 ? sp.gq : sp.gq + sp.gk;
+      const int g1 = kind == 0 ? sp.gq : kind == 1 ? sp.gq + sp.gk : sp.groups;
+      if (g >= g1) continue;
+      const int n = kind == 0 ? dm.nh : dm.nkv;
+      const int first = kind == 0 ? 0 : kind == 1 ? dm.nh : dm.nh + dm.nkv;
+      const float *w = ws + kind * dm.d;
+      F2 a1[V / 2], a2[V / 2];
+      Quad2 w1[V / 4], w2[V / 4];
+      if (kind < 2) {
+        fill(a1, 0.f);
+        fill(a2, 0.f);
+        if (ln.live) {
+#pragma unroll
+          for (int i = 0; i < V / 4; ++i) {
+            w1[i] = quad_at(reinterpret_cast<const float4 *>(w + ln.a) + i);
+            w2[i] = quad_at(reinterpret_cast<const float4 *>(w + ln.b) + i);
+          }
         }
-        ss += y1[e] * y1[e] + y2[e] * y2[e];
-        gx += f1[e] * w1[e] * y1[e] + f2[e] * w2[e] * y2[e];
+      }
+      int left = n - (g - g0) * sp.at_once - ln.slot;
+      char *out = static_cast<char *>(dqkv) + (tok * total + first + (n - left)) * (int64_t)dm.d * es;
+      const char *lora =
+          static_cast<const char *>(lq) + (tok * n + (n - left)) * (int64_t)dm.d * elem_size<L>();
+      for (; g < g1; g += sp.parts) {
+        const bool live = ln.live && left > 0;
+        typename Vec<L, V>::type l1, l2;
+        if (kind == 0 && lq != nullptr && live) {
+          l1 = load_raw<L, V>(lora, ln.a);
+          l2 = load_raw<L, V>(lora, ln.b);
+        }
+        copies_wait<kBwdStages - 2>();
+        F2 f1[V / 2], f2[V / 2];
+        if (live && inside && has[kind]) {
+          Vec<T, V>::get(ring[stage][0][threadIdx.x], f1);
+          Vec<T, V>::get(ring[stage][1][threadIdx.x], f2);
+        } else {
+          fill(f1, 0.f);
+          fill(f2, 0.f);
+        }
+        if (kind < 2) {
+          F2 y1[V / 2], y2[V / 2], dot = both(0.f);
+          float ss = 0.f, gx = 0.f;
+          if (live && inside) {
+            Vec<T, V>::get(ring[stage][2][threadIdx.x], y1);
+            Vec<T, V>::get(ring[stage][3][threadIdx.x], y2);
+            if (kind == 0 && lq != nullptr) {
+              F2 z1[V / 2], z2[V / 2];
+              Vec<L, V>::get(l1, z1);
+              Vec<L, V>::get(l2, z2);
+#pragma unroll
+              for (int i = 0; i < V / 2; ++i) {
+                y1[i] = add2(y1[i], z1[i]);
+                y2[i] = add2(y2[i], z2[i]);
+              }
+            }
+            ss = square_sum(y1, y2);
+            const int next = (V / 4) * sp.lanes;
+#pragma unroll
+            for (int i = 0; i < V / 4; ++i) {
+              const float4 *p = mine + i * sp.lanes;
+              const Quad2 c1 = quad_at(p), s1 = quad_at(p + next), c2 = quad_at(p + 2 * next),
+                          s2 = quad_at(p + 3 * next);
+              const F2 d1 = fma2(f1[2 * i], c1.lo, mul2(f2[2 * i], s2.lo));
+              const F2 e1 = fma2(f1[2 * i + 1], c1.hi, mul2(f2[2 * i + 1], s2.hi));
+              f2[2 * i] = fma2(f2[2 * i], c2.lo, mul2(f1[2 * i], s1.lo));
+              f2[2 * i + 1] = fma2(f2[2 * i + 1], c2.hi, mul2(f1[2 * i + 1], s1.hi));
+              f1[2 * i] = d1;
+              f1[2 * i + 1] = e1;
+              dot = fma2(mul2(d1, y1[2 * i]), w1[i].lo, dot);
+              dot = fma2(mul2(e1, y1[2 * i + 1]), w1[i].hi, dot);
+              dot = fma2(mul2(f2[2 * i], y2[2 * i]), w2[i].lo, dot);
+              dot = fma2(mul2(f2[2 * i + 1], y2[2 * i + 1]), w2[i].hi, dot);
+            }
+            const float2 p = parts(dot);
+            gx = p.x + p.y;
+          }
+          ss = group_sum(ss, sp.lanes);
+          gx = group_sum(gx, sp.lanes);
+          const float r = rsqrtf(fmaf(ss, dm.inv_d, dm.eps));
+          if (live && inside) {
+            const F2 rr = both(r), rk = both(-(r * r * r) * gx * dm.inv_d);
+#pragma unroll
+            for (int i = 0; i < V / 4; ++i) {
+#pragma unroll
+              for (int j = 2 * i; j < 2 * i + 2; ++j) {
+                f1[j] = mul2(f1[j], rr);
+                f2[j] = mul2(f2[j], rr);
+                a1[j] = fma2(f1[j], y1[j], a1[j]);
+                a2[j] = fma2(f2[j], y2[j], a2[j]);
+                f1[j] = fma2(f1[j], j == 2 * i ? w1[i].lo : w1[i].hi, mul2(y1[j], rk));
+                f2[j] = fma2(f2[j], j == 2 * i ? w2[i].lo : w2[i].hi, mul2(y2[j], rk));
+              }
+            }
+          }
+        }
+        fetch((stage + kBwdStages - 1) % kBwdStages);
+        stage = (stage + 1) % kBwdStages;
+        if (live) {
+          *reinterpret_cast<Raw *>(out + ln.a * es) = Vec<T, V>::put(f1);
+          *reinterpret_cast<Raw *>(out + ln.b * es) = Vec<T, V>::put(f2);
+        }
+        left -= step;
+        out += bytes;
+        lora += (int64_t)step * dm.d * elem_size<L>();
+      }
+      if (kind < 2 && ln.live && part != nullptr) {
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+          sums[kind][i][threadIdx.x] = add2(sums[kind][i][threadIdx.x], a1[i]);
+          sums[kind][V / 2 + i][threadIdx.x] = add2(sums[kind][V / 2 + i][threadIdx.x], a2[i]);
+        }
       }
     }
-    ss = group_sum(ss, lanes);
-    gx = group_sum(gx, lanes);
-    if (!live) continue;
-    if (!inside) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) f1[e] = f2[e] = 0.f;
-    } else if (normed) {
-      const float r = rsqrtf(ss * dm.inv_d + dm.eps);
-      const float k2 = r * r * (gx * dm.inv_d);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        a1[e] += f1[e] * y1[e] * r;
-        a2[e] += f2[e] * y2[e] * r;
-        f1[e] = r * (f1[e] * w1[e] - y1[e] * k2);
-        f2[e] = r * (f2[e] * w2[e] - y2[e] * k2);
-      }
-    }
-    const int64_t at = tok * width + (int64_t)hr * dm.d;
-    store4<T>(dqkv, at + ch.a, f1);
-    store4<T>(dqkv, at + ch.b, f2);
   }
+  copies_wait<0>();
   if (part == nullptr) return;
   // the lanes' sums, added in order of the warps and their head rows
-  __shared__ float sums[kThreads][8];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    sums[threadIdx.x][e] = a1[e];
-    sums[threadIdx.x][4 + e] = a2[e];
-  }
   __syncthreads();
-  const int pairs = dm.rot / 8;
+  const int pairs = dm.rot / (2 * V), h = dm.rot / 2;
   for (int i = threadIdx.x; i < 2 * dm.d; i += kThreads) {
-    const int dim = i < dm.d ? i : i - dm.d, h = dm.rot / 2;
-    const int rest = dim - dm.rot;
-    const int at = dim < dm.rot ? (dim % h) / 4 : pairs + rest / 8;
-    const int e = dim < dm.rot ? (dim >= h ? 4 : 0) + dim % 4 : rest % 8;
+    const int dim = i < dm.d ? i : i - dm.d, rest = dim - dm.rot, kind = i < dm.d ? 0 : 1;
+    const int at = dim < dm.rot ? (dim % h) / V : pairs + rest / (2 * V);
+    const int e = dim < dm.rot ? (dim >= h ? V : 0) + dim % V : rest % (2 * V);
     float s = 0.f;
-    for (int w = 0; w < kWarps; ++w) {
-      const int first = ((blockIdx.x * kWarps + w) % groups) * rows_at_once;
-      for (int j = 0; j < rows_at_once; ++j) {
-        const bool isq = first + j < dm.nh, isk = !isq && first + j < dm.nh + dm.nkv;
-        if (i < dm.d ? isq : isk) s += sums[w * 32 + j * lanes + at][e];
-      }
-    }
+    for (int j = 0; j < kThreads / sp.lanes; ++j)
+      s += reinterpret_cast<const float *>(&sums[kind][e / 2][j * sp.lanes + at])[e % 2];
     part[(int64_t)blockIdx.x * 2 * dm.d + i] = s;
   }
 }
@@ -538,34 +789,40 @@ int pow2_at_least(int n) {
   return p;
 }
 
-// Lanes of a head row on the vector path (0: not taken).
-int lanes_of(const NormDims &dm) {
-  if (dm.d % 8 || dm.rot % 8 || dm.d > 256) return 0;
-  return pow2_at_least(dm.d / 8);
+// Dims of a chunk on the vector path (0: not taken): 16 bytes, or 8 where the head size or rot of a
+// 16-bit type ask for it.
+int chunk_of(const NormDims &dm, int type) {
+  if (type != TB_FP32 && dm.d % 16 == 0 && dm.rot % 16 == 0 && dm.d <= 512) return 8;
+  return dm.d % 8 == 0 && dm.rot % 8 == 0 && dm.d <= 256 ? 4 : 0;
 }
 
-int groups_of(const NormDims &dm, int lanes) {
-  const int at_once = 32 / lanes;
-  return (dm.nh + 2 * dm.nkv + at_once - 1) / at_once;
-}
-
-// Warps a token's head rows are spread over in the forward: one when there are many tokens.
-int parts_of(const NormDims &dm, int groups) {
-  const int64_t want = ((int64_t)sm_count() * 32 + dm.rows - 1) / dm.rows;
-  return (int)(want < groups ? want : groups);
-}
-
-// CTAs of the backward: at most the resident ones, whose warps walk the tokens (the vector kernel:
-// at least a warp for each group of head rows; the other: one warp a CTA).
-int bwd_ctas(int64_t rows, int groups) {
-  if (groups == 0) {
-    const int64_t cap = (int64_t)sm_count() * 8;
-    return (int)(rows < cap ? rows : cap);
-  }
-  int64_t cap = (int64_t)sm_count() * 3;
+// CTAs of a walk: `per_sm` resident ones at most, at least a warp for each group of head rows.
+int walk_ctas(const NormDims &dm, int chunk, int per_sm) {
+  const int64_t at_once = 32 / pow2_at_least(dm.d / (2 * chunk));
+  const int64_t groups = (dm.nh + at_once - 1) / at_once + 2 * ((dm.nkv + at_once - 1) / at_once);
+  int64_t cap = (int64_t)sm_count() * per_sm;
   if (cap < (groups + kWarps - 1) / kWarps) cap = (groups + kWarps - 1) / kWarps;
-  const int64_t want = (rows * groups + kWarps - 1) / kWarps;
+  const int64_t want = (dm.rows * groups + kWarps - 1) / kWarps;
   return (int)(want < cap ? want : cap);
+}
+
+// A token's groups over as many warps as `ctas` CTAs have for them.
+Spread spread_of(const NormDims &dm, int chunk, int ctas) {
+  Spread sp;
+  sp.lanes = pow2_at_least(dm.d / (2 * chunk));
+  sp.at_once = 32 / sp.lanes;
+  sp.gq = (dm.nh + sp.at_once - 1) / sp.at_once;
+  sp.gk = (dm.nkv + sp.at_once - 1) / sp.at_once;
+  sp.groups = sp.gq + 2 * sp.gk;
+  const int64_t parts = dm.rows > 0 ? (int64_t)ctas * kWarps / dm.rows : 1;
+  sp.parts = (int)(parts < 1 ? 1 : parts < sp.groups ? parts : sp.groups);
+  return sp;
+}
+
+// CTAs of the backward for any size, one warp each.
+int any_ctas(int64_t rows) {
+  const int64_t cap = (int64_t)sm_count() * 8;
+  return (int)(rows < cap ? rows : cap);
 }
 
 int check(const char *what, const NormDims &dm, int64_t batch, int64_t seq, int type, int l_type,
@@ -587,6 +844,42 @@ int check(const char *what, const NormDims &dm, int64_t batch, int64_t seq, int 
     return set_error(TB_EINVAL, "%s: types %d %d %d", what, type, l_type, w_type);
   return TB_OK;
 }
+
+// Shared memory beyond 48 KB has to be asked for, on every device.
+template <typename Kernel>
+int allow_smem(const char *what, Kernel kernel, size_t bytes) {
+  if (bytes <= 48 * 1024 || cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 (int)bytes) == cudaSuccess)
+    return TB_OK;
+  (void)cudaGetLastError();
+  return set_error(TB_ELAUNCH, "%s: %d bytes of shared memory", what, (int)bytes);
+}
+
+// Runs RUN(T, V, L, W) for the element type, the chunk and the LoRA rows' and weights' types.
+#define TB_WITH_CHUNK(RUN)                                     \
+  do {                                                         \
+    if (type == TB_FP32) {                                     \
+      RUN(TB_FP32, 4, TB_FP32, TB_FP32);                       \
+    } else if (type == TB_FP16) {                              \
+      TB_WITH_PARTS(RUN, TB_FP16);                             \
+    } else {                                                   \
+      TB_WITH_PARTS(RUN, TB_BF16);                             \
+    }                                                          \
+  } while (0)
+#define TB_WITH_PARTS(RUN, T)                                  \
+  do {                                                         \
+    if (chunk == 8) {                                          \
+      if (l_own && w_own) RUN(T, 8, T, T);                     \
+      else if (l_own) RUN(T, 8, T, TB_FP32);                   \
+      else if (w_own) RUN(T, 8, TB_FP32, T);                   \
+      else RUN(T, 8, TB_FP32, TB_FP32);                        \
+    } else {                                                   \
+      if (l_own && w_own) RUN(T, 4, T, T);                     \
+      else if (l_own) RUN(T, 4, T, TB_FP32);                   \
+      else if (w_own) RUN(T, 4, TB_FP32, T);                   \
+      else RUN(T, 4, TB_FP32, TB_FP32);                        \
+    }                                                          \
+  } while (0)
 
 bool all_aligned(std::initializer_list<const void *> ps, uintptr_t a) {
   for (const void *p : ps)
@@ -617,26 +910,28 @@ extern "C" int tb_norm_rope_fwd(const void *qkv, int32_t type, int64_t ld, const
   if (!all_aligned({qkv, q, k, v}, es) || !all_aligned({lora_q, lora_v}, ls) ||
       !all_aligned({q_weight, k_weight}, ws) || !all_aligned({cos, sin}, 4) || !aligned(pos_idx, 8))
     return set_error(TB_EALIGN, "norm_rope_fwd: a buffer is not aligned to its element");
-  const int lanes = lanes_of(dm);
-  const bool vec = lanes > 0 && ld % 4 == 0 && all_aligned({qkv, q, k, v}, 4 * es) &&
-                   all_aligned({lora_q, lora_v}, 4 * ls) &&
-                   all_aligned({q_weight, k_weight}, 4 * ws) && all_aligned({cos, sin}, 16);
+  const int chunk = chunk_of(dm, type);
+  const bool vec = chunk > 0 && ld % chunk == 0 && all_aligned({qkv, q, k, v}, chunk * es) &&
+                   all_aligned({lora_q, lora_v, q_weight, k_weight, cos, sin}, 16);
   cudaStream_t st = as_stream(stream);
   // the LoRA rows and the weights in qkv's type or fp32 on the vector path
   const bool l_own = lora_type == type || (!lora_q && !lora_v);
   const bool w_own = weight_type == type || (!q_weight && !k_weight);
   if (vec && (l_own || lora_type == TB_FP32) && (w_own || weight_type == TB_FP32)) {
     const FastDiv sd((uint32_t)seq);
-    const int parts = parts_of(dm, groups_of(dm, lanes));
-    const int64_t ctas = (rows * parts + kWarps - 1) / kWarps;
-#define TB_FWD(T, L, W)                                                                          \
-  return launch("norm_rope_fwd", norm_rope_fwd<T, L, W>, dim3((unsigned)ctas),                   \
-                kThreads, 0, st, qkv, lora_q, lora_v, q_weight, k_weight, cos, sin, pos_idx, q,  \
-                k, v, dm, sd, FastDiv((uint32_t)parts), lanes)
-    if (l_own && w_own) TB_WITH_TYPE(type, T, TB_FWD(T, T, T));
-    if (l_own) TB_WITH_TYPE(type, T, TB_FWD(T, T, TB_FP32));
-    if (w_own) TB_WITH_TYPE(type, T, TB_FWD(T, TB_FP32, T));
-    TB_WITH_TYPE(type, T, TB_FWD(T, TB_FP32, TB_FP32));
+    const int ctas = walk_ctas(dm, chunk, kFwdPerSm);
+    const Spread sp = spread_of(dm, chunk, ctas);
+#define TB_FWD(T, V, L, W)                                                                       \
+  do {                                                                                           \
+    const size_t kSmem = (size_t)kThreads * kFwdStages * 2 * V * elem_size<T>() +                \
+                         2 * head_dim * 4 + (size_t)kWarps * V * sp.lanes * 16;                  \
+    rc = allow_smem("norm_rope_fwd", norm_rope_fwd<T, V, L, W>, kSmem);                          \
+    if (rc != TB_OK) return rc;                                                                  \
+    return launch("norm_rope_fwd", norm_rope_fwd<T, V, L, W>, dim3((unsigned)ctas), kThreads,    \
+                  kSmem, st, qkv, lora_q, lora_v, q_weight, k_weight, cos, sin, pos_idx, q, k,   \
+                  v, dm, sp, sd);                                                                \
+  } while (0)
+    TB_WITH_CHUNK(TB_FWD);
 #undef TB_FWD
   }
   int64_t blocks = (rows * (n_heads + 2 * (int64_t)n_kv) + 7) / 8;
@@ -652,9 +947,14 @@ extern "C" int64_t tb_norm_rope_bwd_workspace(int64_t rows, int32_t n_heads, int
                                               int32_t head_dim) {
   if (rows <= 0 || n_heads <= 0 || n_kv < 0 || head_dim <= 0) return 0;
   const NormDims dm{rows, 0, 0, n_heads, n_kv, head_dim, 0, 0.f, 0.f, 0.f};
-  const int lanes = lanes_of(dm);
-  const int vec = lanes > 0 ? bwd_ctas(rows, groups_of(dm, lanes)) : 0, any = bwd_ctas(rows, 0);
-  return (int64_t)(vec > any ? vec : any) * 2 * head_dim * 4;
+  // the most of the paths that the type, rot and alignment choose from
+  int most = any_ctas(rows);
+  for (int chunk = 4; chunk <= 8; chunk += 4) {
+    if (head_dim % (2 * chunk) || head_dim > 64 * chunk) continue;
+    const int ctas = walk_ctas(dm, chunk, kBwdPerSm);
+    if (ctas > most) most = ctas;
+  }
+  return (int64_t)most * 2 * head_dim * 4;
 }
 
 extern "C" int tb_norm_rope_bwd(const void *dq, const void *dk, const void *dv, const void *qkv,
@@ -687,27 +987,30 @@ extern "C" int tb_norm_rope_bwd(const void *dq, const void *dk, const void *dv, 
   cudaStream_t st = as_stream(stream);
   int ctas = 0;
   if (rows > 0) {
-    const int lanes = lanes_of(dm);
-    const bool vec = lanes > 0 && ld % 4 == 0 && all_aligned({qkv, dq, dk, dv, dqkv}, 4 * es) &&
-                     aligned(lora_q, 4 * ls) && all_aligned({q_weight, k_weight}, 4 * ws) &&
-                     all_aligned({cos, sin}, 16);
+    const int chunk = chunk_of(dm, type);
+    const bool vec = chunk > 0 && ld % chunk == 0 &&
+                     all_aligned({qkv, dq, dk, dv, dqkv}, chunk * es) &&
+                     all_aligned({lora_q, q_weight, k_weight, cos, sin}, 16);
     const bool l_own = lora_type == type || !lora_q;
     const bool w_own = weight_type == type || (!q_weight && !k_weight);
     if (vec && (l_own || lora_type == TB_FP32) && (w_own || weight_type == TB_FP32)) {
       const FastDiv sd((uint32_t)seq);
-      const int groups = groups_of(dm, lanes);
-      ctas = bwd_ctas(rows, groups);
-#define TB_BWD(T, L, W)                                                                          \
-  rc = launch("norm_rope_bwd", norm_rope_bwd<T, L, W>, dim3((unsigned)ctas), kThreads, 0, st, dq, \
-              dk, dv, qkv, lora_q, q_weight, k_weight, cos, sin, pos_idx, dqkv, part, dm, sd,     \
-              lanes, groups)
-      if (l_own && w_own) TB_WITH_TYPE(type, T, TB_BWD(T, T, T));
-      else if (l_own) TB_WITH_TYPE(type, T, TB_BWD(T, T, TB_FP32));
-      else if (w_own) TB_WITH_TYPE(type, T, TB_BWD(T, TB_FP32, T));
-      else TB_WITH_TYPE(type, T, TB_BWD(T, TB_FP32, TB_FP32));
+      ctas = walk_ctas(dm, chunk, kBwdPerSm);
+      const Spread sp = spread_of(dm, chunk, ctas);
+#define TB_BWD(T, V, L, W)                                                                       \
+  do {                                                                                           \
+    const size_t kSmem = (size_t)kThreads * (kBwdStages * 4 * V * elem_size<T>() + 2 * V * 8) +  \
+                         2 * head_dim * 4 + (size_t)kWarps * V * sp.lanes * 16;                  \
+    rc = allow_smem("norm_rope_bwd", norm_rope_bwd<T, V, L, W>, kSmem);                          \
+    if (rc != TB_OK) return rc;                                                                  \
+    rc = launch("norm_rope_bwd", norm_rope_bwd<T, V, L, W>, dim3((unsigned)ctas), kThreads,      \
+                kSmem, st, dq, dk, dv, qkv, lora_q, q_weight, k_weight, cos, sin, pos_idx, dqkv, \
+                part, dm, sp, sd);                                                               \
+  } while (0)
+      TB_WITH_CHUNK(TB_BWD);
 #undef TB_BWD
     } else {
-      ctas = bwd_ctas(rows, 0);
+      ctas = any_ctas(rows);
       TB_WITH_TYPE(type, T,
                    rc = launch("norm_rope_bwd", norm_rope_bwd_any<T>, dim3((unsigned)ctas), 32,
                                (size_t)2 * head_dim * 4, st, dq, dk, dv, qkv, lora_q, lora_type,
