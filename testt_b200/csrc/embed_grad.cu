@@ -11,9 +11,9 @@
 // a slice, adds rows in fp32 while the id stays, and writes an id's row when it ends. An id that
 // crosses chunks leaves one fp32 partial row per chunk, which the join kernel adds in the order of
 // the chunks. So each dy row is read once, each dW row is rounded once and no float atomics run.
-// Rows of ids without tokens are zeros, written by the CTAs of the sort launches that do not
-// sort (the dense gradient's zeros are most of its bytes: [151936, 1536] fp16 is 467 MB, against
-// 621 tokens' 2 MB), so the sort costs no time of its own. With accumulate set nothing is zeroed
+// Rows of ids without tokens are zeros. The sum launch writes them too, with CTAs of their own that
+// look the ids with tokens up in the sorted keys: they are most of the dense gradient's bytes
+// ([151936, 1536] fp16 is 467 MB, against 621 tokens' 2 MB). With accumulate set nothing is zeroed
 // and the sums are added to what dW holds.
 //
 // Reference: solution/model.py:220-225 embeds the real tokens with a frozen table.
@@ -23,105 +23,185 @@ namespace tb {
 namespace {
 
 constexpr int kTile = 2048;         // keys of one shared-memory sort
-constexpr int kSortThreads = 512;
+constexpr int kSortThreads = 1024;
+constexpr int kFwdPerSm = 4;        // resident CTAs of the forward (5, at 48 registers: 45 against 33 us)
 constexpr int kWays = 16;           // runs merged per launch
+constexpr int kSample = 64;         // sampled keys of a run in a merge
 constexpr int kSumThreads = 256;
+constexpr int kFillRows = 32;       // ids whose zero rows a CTA looks for at a time
+constexpr int64_t kSortClears = 40 << 20, kMergeClears = 64 << 20;  // bytes cleared meanwhile
+constexpr int kMaxChunk = 32;       // places of the sorted order a CTA sums
 constexpr uint64_t kNoKey = ~0ull;  // padding of the last tile
 
 __device__ unsigned int g_invalid = 0;
 
-struct Fill {  // the share of the zero fill of one launch: 16-byte words [lo, hi) and byte edges
+// The first place of the sorted keys whose id is at least `id`, by a warp: 32 probes a round.
+__device__ __forceinline__ int64_t place_of(const uint64_t *keys, int64_t n, int64_t id) {
+  const int lane = threadIdx.x & 31;
+  int64_t lo = 0, hi = n;  // keys below lo are smaller, keys from hi on are not
+  while (lo < hi) {
+    const int64_t step = (hi - lo + 31) / 32, at = lo + lane * step;
+    const bool smaller = at < hi && (int64_t)(__ldg(keys + at) >> 32) < id;
+    const int found = __popc(__ballot_sync(0xffffffffu, smaller));
+    if (found == 0) return lo;
+    const int64_t last = lo + (found - 1) * step;  // the last probe that is smaller
+    lo = last + 1;
+    if (last + step < hi) hi = last + step;
+  }
+  return lo;
+}
+
+// The first rows of the gradient, [lo, hi) in bytes, that a launch of the sort clears with its CTAs
+// from `first` on, before it is known which of them have tokens (the sums overwrite those): enough
+// to hide the sort behind.
+struct Early {
   uint8_t *base;
-  int64_t bytes, lo, hi;
+  int64_t lo, hi;
 };
 
-// Zeros by the CTAs [first, gridDim): words of 16 bytes from the first aligned address; the
-// unaligned edges by the launch that has lo == 0.
-__device__ __forceinline__ void zero_fill(const Fill &f, int first) {
-  if (f.base == nullptr) return;
-  const int64_t head = (16 - (int64_t)(reinterpret_cast<uintptr_t>(f.base) & 15)) & 15;
-  uint4 *words = reinterpret_cast<uint4 *>(f.base + head);
-  const int64_t nw = f.bytes > head ? (f.bytes - head) / 16 : 0;
-  const int64_t me = (int64_t)(blockIdx.x - first) * blockDim.x + threadIdx.x;
-  const int64_t all = (int64_t)(gridDim.x - first) * blockDim.x;
-  const uint4 z = make_uint4(0, 0, 0, 0);
-  for (int64_t i = f.lo + me; i < f.hi && i < nw; i += all) words[i] = z;
-  if (f.lo == 0 && me < 16) {
-    if (me < head && me < f.bytes) f.base[me] = 0;
-    const int64_t tail = head + nw * 16 + me;
-    if (tail < f.bytes) f.base[tail] = 0;
-  }
+__device__ __forceinline__ void clear_early(const Early &e, int me, int all) {
+  uint8_t *p = e.base + e.lo;
+  const int64_t bytes = e.hi - e.lo;
+  int64_t head = (16 - (int64_t)(reinterpret_cast<uintptr_t>(p) & 15)) & 15;
+  if (head > bytes) head = bytes;
+  const int64_t words = (bytes - head) / 16, tail = bytes - head - words * 16;
+  uint4 *w = reinterpret_cast<uint4 *>(p + head);
+  const int64_t step = (int64_t)all * blockDim.x;
+  for (int64_t i = (int64_t)me * blockDim.x + threadIdx.x; i < words; i += step)
+    w[i] = make_uint4(0, 0, 0, 0);
+  if (me == 0 && threadIdx.x < head) p[threadIdx.x] = 0;
+  if (me == 0 && threadIdx.x < tail) p[bytes - tail + threadIdx.x] = 0;
 }
 
+// A token's id in the sort: ids without a gradient sort behind all others, as id `vocab`.
 template <typename I>
-__device__ __forceinline__ uint64_t key_of(const I *ids, int64_t t, int64_t vocab, int64_t pad) {
+__device__ __forceinline__ int64_t sort_id(const I *ids, int64_t t, int64_t vocab, int64_t pad) {
   const int64_t id = (int64_t)ids[t];
-  // ids without a gradient sort behind all others, as id `vocab`
-  const uint64_t v = id < 0 || id >= vocab || id == pad ? (uint64_t)vocab : (uint64_t)id;
-  return v << 32 | (uint64_t)t;
+  return id < 0 || id >= vocab || id == pad ? vocab : id;
 }
 
-// CTAs [0, tiles) sort a tile each; the others fill zeros.
-template <typename I>
+// One step of a bitonic network over the warp's lanes.
+template <typename K>
+__device__ __forceinline__ K lane_step(K k, int lane, int size, int stride) {
+  const K o = __shfl_xor_sync(0xffffffffu, k, stride);
+  const bool up = (lane & size) == 0 || size == 32, lower = (lane & stride) == 0;
+  return (up == lower) == (k < o) ? k : o;
+}
+
+// A CTA a tile of kTile tokens. Inside a tile the keys are (id, place in the tile): in 32 bits (K =
+// uint32_t) where the vocabulary is below 2^21 - 1, else in 64. Each warp sorts runs of 32 in its lanes,
+// then neighbouring runs are merged by ranks in shared memory (a key's place is its place in its run
+// plus the smaller keys of the other, by bisection). The 66-step bitonic network over 2048 keys took
+// 21 us for any number of tokens.
+template <typename I, typename K>
 __global__ void __launch_bounds__(kSortThreads)
     sort_tiles(const I *__restrict__ ids, int64_t n, int64_t vocab, int64_t pad,
-               uint64_t *__restrict__ keys, int tiles, Fill fill) {
+               uint64_t *__restrict__ keys, int tiles, Early early) {
   pdl_wait();
   pdl_release();
   if ((int)blockIdx.x >= tiles) {
-    zero_fill(fill, tiles);
+    clear_early(early, (int)blockIdx.x - tiles, (int)gridDim.x - tiles);
     return;
   }
-  __shared__ uint64_t s[kTile];
+  constexpr int kEach = kTile / kSortThreads, kBits = 11;
+  constexpr K kPad = (K)(sizeof(K) == 4 ? 0x1fffffu : 0xffffffffull) << kBits;
+  static_assert(kTile == 1 << kBits, "a place in the tile has kBits bits");
+  __shared__ K buf[2][kTile];
+  const int lane = threadIdx.x & 31;
   const int64_t base = (int64_t)blockIdx.x * kTile;
-  for (int i = threadIdx.x; i < kTile; i += kSortThreads)
-    s[i] = base + i < n ? key_of(ids, base + i, vocab, pad) : kNoKey;
-  __syncthreads();
-  for (int size = 2; size <= kTile; size *= 2) {
-    for (int stride = size / 2; stride > 0; stride /= 2) {
-      for (int p = threadIdx.x; p < kTile / 2; p += kSortThreads) {
-        const int i = 2 * p - (p & (stride - 1)), j = i + stride;
-        const bool up = (i & size) == 0;
-        const uint64_t a = s[i], b = s[j];
-        if ((a > b) == up) {
-          s[i] = b;
-          s[j] = a;
-        }
-      }
-      __syncthreads();
-    }
+  const int count = (int)(n - base < kTile ? n - base : kTile);
+  K k[kEach];
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int i = threadIdx.x + e * kSortThreads;
+    k[e] = i < count ? (K)sort_id(ids, base + i, vocab, pad) << kBits | (K)i : kPad | (K)i;
   }
-  for (int i = threadIdx.x; i < kTile && base + i < n; i += kSortThreads) keys[base + i] = s[i];
+#pragma unroll
+  for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+    for (int stride = size / 2; stride > 0; stride /= 2)
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) k[e] = lane_step(k[e], lane, size, stride);
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) buf[0][threadIdx.x + e * kSortThreads] = k[e];
+  __syncthreads();
+  int from = 0;
+  for (int run = 32; run < count; run *= 2) {
+    int place[kEach];
+    const K *other[kEach];
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const int i = threadIdx.x + e * kSortThreads;
+      k[e] = buf[from][i];
+      other[e] = buf[from] + ((i / run) ^ 1) * run;
+      place[e] = 0;
+    }
+    for (int half = run; half > 0; half /= 2)
+#pragma unroll
+      for (int e = 0; e < kEach; ++e)
+        if (place[e] + half <= run && other[e][place[e] + half - 1] < k[e]) place[e] += half;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const int i = threadIdx.x + e * kSortThreads;
+      buf[from ^ 1][i / (2 * run) * (2 * run) + i % run + place[e]] = k[e];
+    }
+    __syncthreads();
+    from ^= 1;
+  }
+  for (int i = threadIdx.x; i < count; i += kSortThreads) {
+    const K key = buf[from][i];
+    keys[base + i] = (uint64_t)(key >> kBits) << 32 | (uint64_t)(base + (key & (kTile - 1)));
+  }
 }
 
-// Sorted runs of `run` keys of `in` -> runs of run * kWays keys in `out`. The first `blocks` CTAs
-// merge, the others fill zeros.
+// Sorted runs of `run` (a power of two) keys of `in` -> runs of run * kWays keys in `out`: kWays lanes
+// to a key, a lane counts the smaller keys of one run by bisection, the first steps over a sample of
+// kSample keys of each run in shared memory (the probes, not the latencies, are the cost: one thread
+// a key over all runs took 44 us for 32749 keys, kWays lanes without the sample 22 us). A CTA takes
+// keys of one group of runs only: group blockIdx.y.
 __global__ void __launch_bounds__(256)
-    merge_runs(const uint64_t *__restrict__ in, uint64_t *__restrict__ out, int64_t n, int64_t run,
-               int blocks, Fill fill) {
+    merge_runs(const uint64_t *__restrict__ in, uint64_t *__restrict__ out, int64_t n,
+               int64_t run, int groups, Early early) {
   pdl_wait();
   pdl_release();
-  if ((int)blockIdx.x >= blocks) {
-    zero_fill(fill, blocks);
+  if ((int)blockIdx.y >= groups) {
+    clear_early(early, (int)blockIdx.x, (int)gridDim.x);
     return;
   }
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)blocks * 256) {
-    const uint64_t key = in[i];
-    const int64_t mine = i / run, first = mine / kWays * kWays;
-    int64_t place = first * run + (i - mine * run);
-#pragma unroll 4
-    for (int64_t r = first; r < first + kWays; ++r) {
-      const int64_t lo0 = r * run;
-      if (r == mine || lo0 >= n) continue;
-      int64_t lo = lo0, hi = lo0 + run < n ? lo0 + run : n;
-      while (lo < hi) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (in[mid] < key) lo = mid + 1;
-        else hi = mid;
-      }
-      place += lo - lo0;
+  __shared__ uint64_t sample[kWays][kSample + 1];
+  const int64_t start = (int64_t)blockIdx.y * run * kWays;  // the group's first key
+  const int64_t end = start + run * kWays < n ? start + run * kWays : n;
+  const int64_t each = run / kSample;  // sample j is key (j + 1) each - 1 of its run
+  for (int i = threadIdx.x; i < kWays * kSample; i += 256) {
+    const int r = i / kSample, j = i % kSample;
+    const int64_t at = start + r * run + (j + 1) * each - 1;
+    sample[r][j] = at < end ? in[at] : kNoKey;
+  }
+  __syncthreads();
+  const int lane = threadIdx.x % kWays;
+  const int64_t per = 256 / kWays, all = start + (end - start + per - 1) / per * per;
+  const int64_t lo = start + lane * run;
+  const int64_t len = lo >= end ? 0 : end - lo < run ? end - lo : run;
+  for (int64_t i = start + blockIdx.x * per + threadIdx.x / kWays; i < all;
+       i += (int64_t)gridDim.x * per) {
+    const bool live = i < end;
+    const uint64_t key = live ? in[i] : 0;
+    const int mine = (int)((i - start) / run);
+    int64_t smaller = 0;  // keys of the lane's run known to be smaller
+    if (live && lane == mine) {
+      smaller = i - lo;
+    } else if (live && len > 0) {
+      int s = 0;
+#pragma unroll
+      for (int half = kSample; half > 0; half /= 2)
+        if (s + half <= kSample && sample[lane][s + half - 1] < key) s += half;
+      smaller = s * each;
+      for (int64_t half = each / 2; half > 0; half /= 2)
+        if (smaller + half <= len && in[lo + smaller + half - 1] < key) smaller += half;
     }
-    out[place] = key;
+#pragma unroll
+    for (int o = kWays / 2; o > 0; o /= 2) smaller += __shfl_xor_sync(0xffffffffu, smaller, o);
+    if (live && lane == 0) out[start + smaller] = key;
   }
 }
 
@@ -129,8 +209,9 @@ struct SumArgs {
   const uint64_t *keys;
   const void *dy;
   void *dw;
-  float *part;  // [chunks, 2, hidden]: a chunk's first id (begun before), its last (going on)
-  int64_t n, hidden, vocab;
+  float *part;  // [chunks, 2, wide]: a chunk's first id (begun before), its last (going on)
+  int64_t n, hidden, vocab, wide;  // wide: hidden rounded up to four columns
+  int64_t cleared;  // rows the sort's launches have cleared
   int chunk;
   float scale;
   bool accumulate;
@@ -142,7 +223,7 @@ __device__ __forceinline__ int64_t id_at(const uint64_t *keys, int64_t i, int64_
 
 // Writes an id's finished sum (V columns at c).
 template <int T, int V>
-__device__ __forceinline__ void write_row(const SumArgs &a, int64_t id, int64_t c, float (&f)[8]) {
+__device__ __forceinline__ void write_row(const SumArgs &a, int64_t id, int64_t c, float (&f)[V]) {
   const int64_t at = id * a.hidden + c;
   if constexpr (V == 8) {
     float old[8];
@@ -156,101 +237,322 @@ __device__ __forceinline__ void write_row(const SumArgs &a, int64_t id, int64_t 
   }
 }
 
-// G: dy's type, T: dW's. V columns a thread (8 on 16-byte aligned rows, else 1).
+// V columns of a row as loaded, and their fp32 sums (packed in pairs for V = 8).
+template <int G, int V>
+struct RawRow {
+  using type = typename Elem<G>::type;
+  using Sum = float[1];
+  type v;
+  __device__ __forceinline__ void load(const void *p, int64_t at) {
+    v = __ldg(static_cast<const type *>(p) + at);
+  }
+  __device__ __forceinline__ void add_to(Sum &acc) const { acc[0] += Elem<G>::get(v); }
+  static __device__ __forceinline__ void clear(Sum &acc) { acc[0] = 0.f; }
+  static __device__ __forceinline__ void get(const Sum &acc, float (&f)[1]) { f[0] = acc[0]; }
+};
+
+template <int G>
+struct RawRow<G, 8> {
+  using Sum = F2[4];
+  uint4 v[G == TB_FP32 ? 2 : 1];
+  __device__ __forceinline__ void load(const void *p, int64_t at) {
+    const uint4 *q = reinterpret_cast<const uint4 *>(
+        static_cast<const typename Elem<G>::type *>(p) + at);
+    v[0] = __ldg(q);
+    if constexpr (G == TB_FP32) v[1] = __ldg(q + 1);
+  }
+  __device__ __forceinline__ void add_to(Sum &acc) const {
+    if constexpr (G == TB_FP32) {
+      const float *f = reinterpret_cast<const float *>(v);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] = add2(acc[i], make_f2(f[2 * i], f[2 * i + 1]));
+    } else {
+      const uint32_t *w = reinterpret_cast<const uint32_t *>(v);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = Elem<G>::get2(w[i]);
+        acc[i] = add2(acc[i], make_f2(f.x, f.y));
+      }
+    }
+  }
+  static __device__ __forceinline__ void clear(Sum &acc) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] = both(0.f);
+  }
+  static __device__ __forceinline__ void get(const Sum &acc, float (&f)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 p = parts(acc[i]);
+      f[2 * i] = p.x;
+      f[2 * i + 1] = p.y;
+    }
+  }
+};
+
+// Zeros over `bytes` from p by a warp: 16-byte words between the unaligned edges.
+__device__ __forceinline__ void warp_zero(uint8_t *p, int64_t bytes) {
+  const int lane = threadIdx.x & 31;
+  int64_t head = (16 - (int64_t)(reinterpret_cast<uintptr_t>(p) & 15)) & 15;
+  if (head > bytes) head = bytes;
+  const int64_t words = (bytes - head) / 16, tail = bytes - head - words * 16;
+  uint4 *w = reinterpret_cast<uint4 *>(p + head);
+  for (int64_t i = lane; i < words; i += 32) w[i] = make_uint4(0, 0, 0, 0);
+  if (lane < head) p[lane] = 0;
+  if (lane < tail) p[bytes - tail + lane] = 0;
+}
+
+// The zero rows, kFillRows ids to a CTA at a time: the ids among them that have tokens are marked
+// from the sorted keys, the warps clear the others.
+__device__ __forceinline__ void fill_rows(const SumArgs &a, int row_bytes, int me, int all) {
+  __shared__ uint8_t used[kFillRows];
+  __shared__ int64_t range[2];
+  const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  for (int64_t r0 = a.cleared + (int64_t)me * kFillRows; r0 < a.vocab;
+       r0 += (int64_t)all * kFillRows) {
+    const int count = (int)(a.vocab - r0 < kFillRows ? a.vocab - r0 : kFillRows);
+    for (int i = threadIdx.x; i < kFillRows; i += blockDim.x) used[i] = 0;
+    if (warp < 2) {
+      const int64_t at = place_of(a.keys, a.n, warp == 0 ? r0 : r0 + count);
+      if ((threadIdx.x & 31) == 0) range[warp] = at;
+    }
+    __syncthreads();
+    for (int64_t i = range[0] + threadIdx.x; i < range[1]; i += blockDim.x)
+      used[(int64_t)(__ldg(a.keys + i) >> 32) - r0] = 1;
+    __syncthreads();
+    for (int i = warp; i < count; i += warps)
+      if (!used[i]) warp_zero(static_cast<uint8_t *>(a.dw) + (r0 + i) * row_bytes, row_bytes);
+    __syncthreads();
+  }
+}
+
+// CTAs [0, chunks x slices) sum, the others (`fill_ctas`) fill zeros: both only need the sorted keys
+// and write different rows, so the fill hides the sums' latencies and the sums cost their bytes.
+// G: dy's type, T: dW's. V columns a thread (8 on 16-byte aligned rows, else 1); kAhead rows of dy
+// in flight, whatever ids they belong to.
 template <int G, int T, int V>
-__global__ void __launch_bounds__(kSumThreads) sum_chunks(SumArgs a) {
+__global__ void __launch_bounds__(kSumThreads) sum_chunks(SumArgs a, int chunks, int sums) {
   pdl_wait();
   pdl_release();
-  const int64_t p0 = (int64_t)blockIdx.x * a.chunk;
-  const int64_t p1 = p0 + a.chunk < a.n ? p0 + a.chunk : a.n;
-  const int64_t c = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * V;
-  if (c >= a.hidden) return;
-  const int64_t before = id_at(a.keys, p0 - 1, a.n), after = id_at(a.keys, p1, a.n);
-  const int64_t first = id_at(a.keys, p0, a.n);
-  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  int64_t id = first;
-  bool earlier = before == first;  // the running id began in an earlier chunk
-  for (int64_t p = p0; p < p1; ++p) {
+  // the fill's CTAs are spread among the others: fills(b) of the first b CTAs
+  const int64_t fill = (int64_t)gridDim.x - sums;
+  const int before = (int)(fill * blockIdx.x / gridDim.x);
+  if ((int)(fill * (blockIdx.x + 1) / gridDim.x) != before) {
+    fill_rows(a, (int)a.hidden * elem_size<T>(), before, (int)fill);
+    return;
+  }
+  constexpr int kAhead = 8;
+  const int me = (int)blockIdx.x - before, slice = me / chunks, chunk = me - slice * chunks;
+  // of the chunk's places: the token, with bit 31 set where its id ends; the id
+  __shared__ uint32_t sh_tok[kMaxChunk];
+  __shared__ uint32_t sh_id[kMaxChunk];
+  __shared__ bool sh_earlier;  // the first id began in an earlier chunk
+  const int64_t p0 = (int64_t)chunk * a.chunk;
+  const int count = (int)(a.n - p0 < a.chunk ? a.n - p0 : a.chunk);
+  for (int i = threadIdx.x; i < count; i += blockDim.x) {
+    const int64_t p = p0 + i;
     const uint64_t key = __ldg(a.keys + p);
-    const int64_t next = p + 1 < p1 ? id_at(a.keys, p + 1, a.n) : after;
-    if (id < a.vocab) {
-      const int64_t at = (int64_t)(key & 0xffffffffu) * a.hidden + c;
-      float f[8];
-      if constexpr (V == 8) load8<G>(a.dy, at, f);
-      else f[0] = load1<G>(a.dy, at);
+    const uint32_t id = (uint32_t)(key >> 32);
+    const bool ends = p + 1 >= a.n || (uint32_t)(__ldg(a.keys + p + 1) >> 32) != id;
+    sh_tok[i] = (uint32_t)key | (ends ? 0x80000000u : 0u);
+    sh_id[i] = id;
+    if (i == 0) sh_earlier = p0 > 0 && (uint32_t)(__ldg(a.keys + p0 - 1) >> 32) == id;
+  }
+  __syncthreads();
+  const int64_t c = ((int64_t)slice * blockDim.x + threadIdx.x) * V;
+  if (c >= a.hidden) return;
+  using Row = RawRow<G, V>;
+  typename Row::Sum acc;
+  Row::clear(acc);
+  bool earlier = sh_earlier;
+  for (int i0 = 0; i0 < count; i0 += kAhead) {
+    Row row[kAhead];
+    const int m = count - i0;
 #pragma unroll
-      for (int e = 0; e < V; ++e) acc[e] += f[e];
-    }
-    const bool ends = next != id;
-    if (ends || p + 1 == p1) {
-      if (id < a.vocab) {
-        if (ends && !earlier) {
-          write_row<T, V>(a, id, c, acc);
+    for (int j = 0; j < kAhead; ++j)
+      if (j < m) row[j].load(a.dy, (int64_t)(sh_tok[i0 + j] & 0x7fffffffu) * a.hidden + c);
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      if (j >= m) break;
+      const bool ends = (sh_tok[i0 + j] & 0x80000000u) != 0;
+      row[j].add_to(acc);
+      if (!ends && i0 + j + 1 < count) continue;
+      const int64_t id = sh_id[i0 + j];
+      if (id >= a.vocab) return;  // the ids without a gradient are the last
+      float f[V];
+      Row::get(acc, f);
+      if (ends && !earlier) {
+        write_row<T, V>(a, id, c, f);
+      } else {
+        float *dst = a.part + ((int64_t)chunk * 2 + (earlier ? 0 : 1)) * a.wide + c;
+        if constexpr (V == 8) {
+          store8f(dst, f);
         } else {
-          float *dst = a.part + ((int64_t)blockIdx.x * 2 + (earlier ? 0 : 1)) * a.hidden + c;
-#pragma unroll
-          for (int e = 0; e < V; ++e) dst[e] = acc[e];
+          dst[0] = f[0];
         }
       }
       earlier = false;
-      id = next;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+      Row::clear(acc);
     }
   }
 }
 
-// The ids that cross chunks: the CTA of the chunk an id begins in adds its partial rows in order.
+// Adds partials i0, i0 + step, ... of `count` to s (partial 0 is the second row of chunk `first`,
+// partial i the first row of chunk first + i), eight in flight.
+__device__ __forceinline__ void add_partials(const SumArgs &a, int64_t first, int64_t count,
+                                             int64_t i0, int step, int64_t c, float4 &s) {
+  constexpr int kAhead = 8;
+  for (; i0 < count; i0 += (int64_t)step * kAhead) {
+    float4 f[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int64_t i = i0 + (int64_t)j * step;
+      f[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i < count)
+        f[j] = *reinterpret_cast<const float4 *>(
+            a.part + ((first + i) * 2 + (i == 0 ? 1 : 0)) * a.wide + c);
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      s.x += f[j].x;
+      s.y += f[j].y;
+      s.z += f[j].z;
+      s.w += f[j].w;
+    }
+  }
+}
+
 template <int T>
-__global__ void __launch_bounds__(kSumThreads) join_chunks(SumArgs a) {
-  pdl_wait();
-  pdl_release();
-  const int64_t chunk = blockIdx.x, p1 = (chunk + 1) * a.chunk;
-  if (p1 >= a.n) return;
-  const int64_t id = id_at(a.keys, p1 - 1, a.n);
-  if (id >= a.vocab || id_at(a.keys, p1, a.n) != id) return;
-  const int64_t p0 = chunk * a.chunk;
-  if (id_at(a.keys, p0, a.n) == id && id_at(a.keys, p0 - 1, a.n) == id) return;  // began earlier
-  // the first place behind the id's
-  int64_t lo = p1, hi = a.n;
-  while (lo < hi) {
-    const int64_t mid = (lo + hi) >> 1;
-    if ((int64_t)(__ldg(a.keys + mid) >> 32) <= id) lo = mid + 1;
-    else hi = mid;
+__device__ __forceinline__ void write_quad(const SumArgs &a, int64_t id, int64_t c, float4 s) {
+  const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float f[1] = {v[e]};
+    if (c + e < a.hidden) write_row<T, 1>(a, id, c + e, f);
   }
-  const int64_t last = (lo - 1) / a.chunk;
-  const int64_t c = (int64_t)blockIdx.y * blockDim.x + threadIdx.x;
-  if (c >= a.hidden) return;
-  float s = a.part[(chunk * 2 + 1) * a.hidden + c];
-  for (int64_t k = chunk + 1; k <= last; ++k) s += a.part[k * 2 * a.hidden + c];
-  float f[8] = {s};
-  write_row<T, 1>(a, id, c, f);
 }
 
-// A group of blockDim.x threads per token over its columns, V at a time.
-template <int T, int O, int V, typename I>
-__global__ void __launch_bounds__(256)
-    embedding_fwd(const I *__restrict__ ids, const void *__restrict__ table, int64_t ld,
-                  void *__restrict__ out, int64_t n, int64_t hidden, int64_t vocab, float scale) {
+// The ids that cross chunks, 128 columns to a CTA. Warp w looks at chunk 8 x + w: whether an id
+// begins in it and goes on, and how far; up to kAlone partial rows it adds itself, in order. Longer
+// ones the CTA adds together afterwards, a warp every eighth row, then the warps' sums in order.
+template <int T>
+__global__ void __launch_bounds__(kSumThreads, 4) join_chunks(SumArgs a, int64_t chunks) {
   pdl_wait();
   pdl_release();
-  for (int64_t t = (int64_t)blockIdx.x * blockDim.y + threadIdx.y; t < n;
-       t += (int64_t)gridDim.x * blockDim.y) {
-    const int64_t id = (int64_t)ids[t];
-    const bool ok = id >= 0 && id < vocab;
-    if (!ok && threadIdx.x == 0) atomicAdd(&g_invalid, 1u);
-    for (int64_t c = (int64_t)threadIdx.x * V; c < hidden; c += (int64_t)blockDim.x * V) {
-      float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if constexpr (V == 8) {
-        if (ok) load8<T>(table, id * ld + c, f);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] *= scale;
-        store8<O>(out, t * hidden + c, f);
-      } else {
-        store1<O>(out, t * hidden + c, ok ? load1<T>(table, id * ld + c) * scale : 0.f);
-      }
+  constexpr int kWarps = kSumThreads / 32, kAlone = 24;
+  __shared__ int64_t sh_id[kWarps], sh_count[kWarps];
+  __shared__ float4 sh_sum[kWarps][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t chunk = (int64_t)blockIdx.x * kWarps + warp;
+  const int64_t c = (int64_t)blockIdx.y * 128 + lane * 4;
+  int64_t id = -1, count = 0;
+  const int64_t p0 = chunk * a.chunk, p1 = p0 + a.chunk;
+  if (chunk < chunks && p1 < a.n) {
+    const int64_t here = id_at(a.keys, p1 - 1, a.n), next = id_at(a.keys, p1, a.n);
+    const int64_t start = id_at(a.keys, p0, a.n), before = id_at(a.keys, p0 - 1, a.n);
+    if (here < a.vocab && next == here && !(start == here && before == here)) {
+      id = here;
+      // most go on into the next chunk only
+      const int64_t behind = id_at(a.keys, p1 + a.chunk, a.n);
+      const int64_t end = behind == id ? place_of(a.keys, a.n, id + 1) : p1 + 1;
+      count = behind == id ? (end - 1) / a.chunk - chunk + 1 : 2;
     }
   }
+  if (lane == 0) {
+    sh_id[warp] = id;
+    sh_count[warp] = count > kAlone ? count : 0;
+  }
+  if (count > 0 && count <= kAlone && c < a.wide) {
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    add_partials(a, chunk, count, 0, 1, c, s);
+    write_quad<T>(a, id, c, s);
+  }
+  __syncthreads();
+  for (int w = 0; w < kWarps; ++w) {
+    if (sh_count[w] == 0) continue;  // for the whole CTA
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (c < a.wide)
+      add_partials(a, (int64_t)blockIdx.x * kWarps + w, sh_count[w], warp, kWarps, c, s);
+    sh_sum[warp][lane] = s;
+    __syncthreads();
+    if (warp == 0) {
+      for (int i = 1; i < kWarps; ++i) {
+        const float4 o = sh_sum[i][lane];
+        s.x += o.x;
+        s.y += o.y;
+        s.z += o.z;
+        s.w += o.w;
+      }
+      if (c < a.wide) write_quad<T>(a, sh_id[w], c, s);
+    }
+    __syncthreads();
+  }
+}
+
+// Vectors of V columns, numbered through the tokens (`cols` to a token), kAhead in flight a thread;
+// the next ones' ids are on their way meanwhile.
+template <int T, int O, int V, int kAhead, typename I>
+__global__ void __launch_bounds__(256, kAhead == 1 ? 8 : kFwdPerSm)
+    embedding_fwd(const I *__restrict__ ids, const void *__restrict__ table, int64_t ld,
+                  void *__restrict__ out, uint32_t all, FastDiv cols, int64_t hidden,
+                  int64_t vocab, float scale) {
+  pdl_wait();
+  pdl_release();
+  uint32_t tok[kAhead], vec[kAhead];
+  I id[kAhead];
+  auto look = [&](uint32_t first) {
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const uint32_t i = first + j * 256;
+      cols.divmod(i < all ? i : 0, tok[j], vec[j]);
+      id[j] = i < all ? __ldg(ids + tok[j]) : (I)-1;
+    }
+  };
+  const uint32_t step = gridDim.x * 256 * kAhead;
+  uint32_t first = blockIdx.x * 256 * kAhead + threadIdx.x;
+  look(first);
+  while (first < all) {
+    RawRow<T, V> row[kAhead];
+    int64_t at[kAhead];
+    bool ok[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      ok[j] = id[j] >= 0 && (int64_t)id[j] < vocab;
+      at[j] = (int64_t)tok[j] * hidden + vec[j] * V;
+      if (ok[j]) row[j].load(table, (int64_t)id[j] * ld + vec[j] * V);
+      else if (first + j * 256 < all && vec[j] == 0) atomicAdd(&g_invalid, 1u);
+    }
+    const uint32_t now = first;
+    first = all - first > step ? first + step : all;
+    look(first);
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      if (now + j * 256 >= all) break;
+      typename RawRow<T, V>::Sum sum;
+      RawRow<T, V>::clear(sum);
+      if (ok[j]) row[j].add_to(sum);
+      float f[V];
+      RawRow<T, V>::get(sum, f);
+#pragma unroll
+      for (int e = 0; e < V; ++e) f[e] *= scale;
+      if constexpr (V == 8) store8<O>(out, at[j], f);
+      else store1<O>(out, at[j], f[0]);
+    }
+  }
+}
+
+template <int T, int O, int V, typename I>
+int launch_fwd(const I *ids, const void *table, int64_t ld, void *out, int64_t all, int64_t cols,
+               int64_t hidden, int64_t vocab, float scale, cudaStream_t st) {
+  const FastDiv fd((uint32_t)cols);
+  const int64_t resident = (int64_t)sm_count() * 8 * 256;
+  if (all <= resident)  // a vector a thread when that does not fill the device
+    return launch("embedding_fwd", embedding_fwd<T, O, V, 1, I>, dim3((unsigned)((all + 255) / 256)),
+                  256, 0, st, ids, table, ld, out, (uint32_t)all, fd, hidden, vocab, scale);
+  int64_t blocks = (all + 1023) / 1024;
+  const int64_t cap = (int64_t)sm_count() * kFwdPerSm;
+  if (blocks > cap) blocks = cap;
+  return launch("embedding_fwd", embedding_fwd<T, O, V, 4, I>, dim3((unsigned)blocks), 256, 0, st,
+                ids, table, ld, out, (uint32_t)all, fd, hidden, vocab, scale);
 }
 
 template <int T, int O, typename I>
@@ -259,24 +561,22 @@ int run_fwd(const I *ids, const void *table, int64_t ld, void *out, int64_t n, i
   const bool vec = hidden % 8 == 0 && aligned(table, 16) && aligned(out, 16) &&
                    ld * elem_size<T>() % 16 == 0;
   const int64_t cols = vec ? hidden / 8 : hidden;
-  const int64_t passes = (cols + 255) / 256;
-  const int tx = (int)((cols + passes - 1) / passes), ty = 256 / tx;
-  int64_t blocks = (n + ty - 1) / ty;
-  const int64_t cap = (int64_t)sm_count() * 32;
-  if (blocks > cap) blocks = cap;
-  const dim3 grid((unsigned)blocks), block(tx, ty);
-  if (vec)
-    return launch("embedding_fwd", embedding_fwd<T, O, 8, I>, grid, block, 0, st, ids, table, ld,
-                  out, n, hidden, vocab, scale);
-  return launch("embedding_fwd", embedding_fwd<T, O, 1, I>, grid, block, 0, st, ids, table, ld,
-                out, n, hidden, vocab, scale);
+  const int64_t most = 0x7fff0000LL / cols;  // tokens a launch numbers in 32 bits
+  for (int64_t t = 0; t < n; t += most) {
+    const int64_t all = (n - t < most ? n - t : most) * cols;
+    void *o = static_cast<char *>(out) + t * hidden * elem_size<O>();
+    const int rc = vec ? launch_fwd<T, O, 8>(ids + t, table, ld, o, all, cols, hidden, vocab, scale, st)
+                       : launch_fwd<T, O, 1>(ids + t, table, ld, o, all, cols, hidden, vocab, scale, st);
+    if (rc != TB_OK) return rc;
+  }
+  return TB_OK;
 }
 
-// Places of the sorted order a CTA sums: enough CTAs for the device, 32 places at most.
-int chunk_of(int64_t n) { return n >= 32768 ? 32 : n >= 8192 ? 16 : 8; }
+// Places of the sorted order a CTA sums: two or more CTAs an SM where there are as many tokens.
+int chunk_of(int64_t n) { return n >= 16384 ? kMaxChunk : n >= 8192 ? 16 : 8; }
 
 struct GradPlan {
-  int64_t tiles, chunks, keys_bytes, part_bytes;
+  int64_t tiles, chunks, keys_bytes, part_bytes, wide;
   int chunk, merges;
 };
 
@@ -288,8 +588,20 @@ GradPlan grad_plan(int64_t n, int64_t hidden) {
   p.merges = 0;
   for (int64_t run = kTile; run < n; run *= kWays) ++p.merges;
   p.keys_bytes = (n * 8 + 15) / 16 * 16;
-  p.part_bytes = p.chunks * 2 * hidden * 4;
+  p.wide = (hidden + 3) / 4 * 4;
+  p.part_bytes = p.chunks * 2 * p.wide * 4;
   return p;
+}
+
+template <typename I>
+int run_sort(const I *ids, int64_t n, int64_t vocab, int64_t pad, uint64_t *keys, int64_t tiles,
+             const Early &early, cudaStream_t st) {
+  const dim3 grid((unsigned)(tiles + (early.hi > early.lo ? sm_count() : 0)));
+  if (vocab < (1 << 21) - 1)
+    return launch("embedding_grad", sort_tiles<I, uint32_t>, grid, kSortThreads, 0, st, ids, n,
+                  vocab, pad, keys, (int)tiles, early);
+  return launch("embedding_grad", sort_tiles<I, uint64_t>, grid, kSortThreads, 0, st, ids, n, vocab,
+                pad, keys, (int)tiles, early);
 }
 
 template <int G, int T>
@@ -299,12 +611,27 @@ int run_sums(const SumArgs &a, int64_t chunks, cudaStream_t st) {
   const int64_t slices = (cols + kSumThreads - 1) / kSumThreads;
   int threads = (int)((cols + slices - 1) / slices);
   threads = (threads + 31) / 32 * 32;
-  const dim3 grid((unsigned)chunks, (unsigned)slices);
-  int rc = vec ? launch("embedding_grad", sum_chunks<G, T, 8>, grid, threads, 0, st, a)
-               : launch("embedding_grad", sum_chunks<G, T, 1>, grid, threads, 0, st, a);
-  if (rc != TB_OK || chunks == 1) return rc;
-  const dim3 jgrid((unsigned)chunks, (unsigned)((a.hidden + kSumThreads - 1) / kSumThreads));
-  return launch("embedding_grad", join_chunks<T>, jgrid, kSumThreads, 0, st, a);
+  if (threads < 64) threads = 64;  // two warps look for the fill's ids
+  const int64_t sums = chunks * slices;
+  // the fill: enough resident CTAs to run at the memory's rate, fewer when there are few rows
+  int64_t fill = 0;
+  if (!a.accumulate) {
+    fill = (int64_t)sm_count() * (1024 / threads);
+    const int64_t units = (a.vocab - a.cleared + kFillRows - 1) / kFillRows;
+    if (fill > units) fill = units;
+  }
+  if (sums + fill > 0x7fffffffLL)
+    return set_error(TB_EINVAL, "embedding_grad: %lld tokens of %lld columns", (long long)a.n,
+                     (long long)a.hidden);
+  if (sums + fill == 0) return TB_OK;
+  const dim3 grid((unsigned)(sums + fill));
+  int rc = vec ? launch("embedding_grad", sum_chunks<G, T, 8>, grid, threads, 0, st, a, (int)chunks,
+                        (int)sums)
+               : launch("embedding_grad", sum_chunks<G, T, 1>, grid, threads, 0, st, a, (int)chunks,
+                        (int)sums);
+  if (rc != TB_OK || chunks <= 1) return rc;
+  const dim3 jgrid((unsigned)((chunks + 7) / 8), (unsigned)((a.hidden + 127) / 128));
+  return launch("embedding_grad", join_chunks<T>, jgrid, kSumThreads, 0, st, a, chunks);
 }
 
 int check_sizes(const char *what, int64_t n, int64_t hidden, int64_t vocab) {
@@ -384,40 +711,40 @@ extern "C" int tb_embedding_grad(const void *ids, int32_t ids_int64, const void 
   uint8_t *ws = static_cast<uint8_t *>(workspace);
   uint64_t *keys = reinterpret_cast<uint64_t *>(ws);
   uint64_t *other = reinterpret_cast<uint64_t *>(ws + p.keys_bytes);
-  Fill fill{accumulate ? nullptr : static_cast<uint8_t *>(dw), vocab * hidden * es, 0, 0};
-  const int64_t words = fill.bytes / 16 + 1;
-  const int fill_ctas = accumulate ? 0 : sm_count() * 4;
-  // the zero fill in equal shares over the sort's launches
-  const int launches = 1 + p.merges;
-  int64_t share = 0;
-  auto next_share = [&]() {
-    fill.lo = words * share / launches;
-    fill.hi = words * ++share / launches;
+  // rows the sort's launches clear, whole ones
+  const int64_t row_bytes = hidden * es;
+  int64_t cleared = 0;
+  Early early{static_cast<uint8_t *>(dw), 0, 0};
+  auto clear_rows = [&](int64_t bytes) {
+    early.lo = cleared * row_bytes;
+    if (!accumulate) cleared = cleared + bytes / row_bytes < vocab ? cleared + bytes / row_bytes : vocab;
+    early.hi = cleared * row_bytes;
   };
-  next_share();
-  const dim3 grid((unsigned)(p.tiles + fill_ctas));
-  if (grid.x == 0) return TB_OK;
-  if (ids_int64)
-    rc = launch("embedding_grad", sort_tiles<int64_t>, grid, kSortThreads, 0, st,
-                static_cast<const int64_t *>(ids), n, vocab, padding_idx, keys, (int)p.tiles, fill);
-  else
-    rc = launch("embedding_grad", sort_tiles<int32_t>, grid, kSortThreads, 0, st,
-                static_cast<const int32_t *>(ids), n, vocab, padding_idx, keys, (int)p.tiles, fill);
-  if (rc != TB_OK || n == 0) return rc;
+  if (n > 0) {
+    clear_rows(kSortClears);
+    rc = ids_int64
+             ? run_sort(static_cast<const int64_t *>(ids), n, vocab, padding_idx, keys, p.tiles, early,
+                        st)
+             : run_sort(static_cast<const int32_t *>(ids), n, vocab, padding_idx, keys, p.tiles, early,
+                        st);
+    if (rc != TB_OK) return rc;
+  }
   for (int64_t run = kTile; run < n; run *= kWays) {
-    next_share();
-    int64_t blocks = (n + 255) / 256;
-    const int64_t cap = (int64_t)sm_count() * 8;
+    const int64_t group = run * kWays, groups = (n + group - 1) / group;
+    int64_t blocks = ((n < group ? n : group) * kWays + 255) / 256;
+    const int64_t cap = (int64_t)sm_count() * 8 / groups + 1;
     if (blocks > cap) blocks = cap;
-    rc = launch("embedding_grad", merge_runs, dim3((unsigned)(blocks + fill_ctas)), 256, 0, st,
-                keys, other, n, run, (int)blocks, fill);
+    clear_rows(kMergeClears);
+    rc = launch("embedding_grad", merge_runs,
+                dim3((unsigned)blocks, (unsigned)(groups + (early.hi > early.lo ? 1 : 0))), 256, 0,
+                st, keys, other, n, run, (int)groups, early);
     if (rc != TB_OK) return rc;
     uint64_t *t = keys;
     keys = other;
     other = t;
   }
   const SumArgs a{keys,  dy,    dw,      reinterpret_cast<float *>(ws + 2 * p.keys_bytes),
-                  n,     hidden, vocab, p.chunk, scale, accumulate != 0};
+                  n,     hidden, vocab, p.wide, cleared, p.chunk, scale, accumulate != 0};
 #define TB_SUM(G, T) return run_sums<G, T>(a, p.chunks, st)
   if (dy_type == type) TB_WITH_TYPE(type, T, TB_SUM(T, T));
   if (dy_type == TB_FP32) TB_WITH_TYPE(type, T, TB_SUM(TB_FP32, T));
