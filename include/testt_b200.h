@@ -612,7 +612,7 @@ int tb_embedding_grad(const void *ids, int32_t ids_int64, const void *dy, int32_
                       int64_t n, int64_t hidden, int64_t vocab, void *workspace,
                       int64_t workspace_bytes, void *stream);
 
-/* Bytes of workspace tb_embedding_grad needs. */
+/* Bytes of workspace tb_embedding_grad needs (0, and a NULL workspace, up to 256 tokens). */
 int64_t tb_embedding_grad_workspace(int64_t n, int64_t hidden);
 
 /* Log-probabilities of given tokens, entropy and the top alternatives of logits / temperature in

@@ -44,7 +44,9 @@ def _check_grad(got, ids, dy, vocab, scale, pad=None, old=None, what=""):
 @pytest.mark.parametrize("n,vocab,hidden,kind", [
     (1, 1, 1, "same"), (1, 17, 8, "uniform"), (7, 5, 65, "uniform"), (621, 1000, 136, "zipf"),
     (2048, 31, 24, "uniform"), (2049, 300, 8, "zipf"), (5000, 40, 40, "same"),
-    (9001, 2000, 72, "zipf"), (300, 11, 4104, "zipf"), (40, 70000, 33, "uniform")])
+    (9001, 2000, 72, "zipf"), (300, 11, 4104, "zipf"), (40, 70000, 33, "uniform"),
+    (256, 90, 40, "zipf"), (257, 90, 40, "zipf"), (255, 3, 2112, "same"), (64, 64, 16, "uniform"),
+    (65, 500, 9, "zipf"), (33, 40, 264, "uniform")])
 def test_forward_and_gradient(n, vocab, hidden, kind, dtype):
     from testt_b200.embed import embedding
 
@@ -139,14 +141,18 @@ def test_unaligned_gradient_rows_keep_their_neighbours():
             dw = buf[lead:lead + vocab * hidden]
             ids = torch.tensor([1, 2, 1], device=DEV)
             dy = torch.ones(3, hidden, dtype=torch.float16, device=DEV)
-            nbytes = _lib.load().tb_embedding_grad_workspace(3, hidden)
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=DEV)
-            _lib.call("tb_embedding_grad", _lib.ptr(ids), 1, _lib.ptr(dy), 0, _lib.ptr(dw), 0, 1.0,
-                      -1, 0, 3, hidden, vocab, _lib.ptr(ws), nbytes, _lib.stream_of(dw))
             want = torch.zeros(vocab, hidden)
             want[1], want[2] = 2, 1
-            assert torch.equal(dw.cpu().float().view(vocab, hidden), want)
-            assert torch.all(buf[:lead] == 7) and torch.all(buf[lead + vocab * hidden:] == 7)
+            for copies in (1, 100):  # one launch; the sort, the sums and the join
+                n, dw_of = 3 * copies, dw.fill_(9.0)
+                nbytes = _lib.load().tb_embedding_grad_workspace(n, hidden)
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=DEV) if nbytes else None
+                many, rows = ids.repeat(copies), dy.repeat(copies, 1)
+                _lib.call("tb_embedding_grad", _lib.ptr(many), 1, _lib.ptr(rows), 0,
+                          _lib.ptr(dw_of), 0, 1.0, -1, 0, n, hidden, vocab, _lib.ptr(ws), nbytes,
+                          _lib.stream_of(dw))
+                assert torch.equal(dw.cpu().float().view(vocab, hidden), want * copies)
+                assert torch.all(buf[:lead] == 7) and torch.all(buf[lead + vocab * hidden:] == 7)
 
 
 def test_no_tokens_and_same_bits():

@@ -28,6 +28,7 @@ constexpr int kFwdPerSm = 4;        // resident CTAs of the forward (5, at 48 re
 constexpr int kWays = 16;           // runs merged per launch
 constexpr int kSample = 64;         // sampled keys of a run in a merge
 constexpr int kSumThreads = 256;
+constexpr int kSmall = 256;         // tokens the one-launch gradient takes
 constexpr int kFillRows = 32;       // ids whose zero rows a CTA looks for at a time
 constexpr int64_t kSortClears = 40 << 20, kMergeClears = 64 << 20;  // bytes cleared meanwhile
 constexpr int kMaxChunk = 32;       // places of the sorted order a CTA sums
@@ -325,10 +326,52 @@ __device__ __forceinline__ void fill_rows(const SumArgs &a, int row_bytes, int m
   }
 }
 
+// Adds the rows of places [from, to) while their id stays, kAhead rows of dy in flight whatever ids
+// they belong to, and writes each id's row where it ends (tok has bit 31 set there), or a partial
+// row of the chunk. earlier: the first id began in an earlier chunk.
+template <int G, int T, int V>
+__device__ __forceinline__ void sum_places(const SumArgs &a, const uint32_t *tok,
+                                           const uint32_t *ids, int from, int to, bool earlier,
+                                           int chunk, int64_t c) {
+  constexpr int kAhead = 8;
+  using Row = RawRow<G, V>;
+  typename Row::Sum acc;
+  Row::clear(acc);
+  for (int i0 = from; i0 < to; i0 += kAhead) {
+    Row row[kAhead];
+    const int m = to - i0;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (j < m) row[j].load(a.dy, (int64_t)(tok[i0 + j] & 0x7fffffffu) * a.hidden + c);
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      if (j >= m) break;
+      const bool ends = (tok[i0 + j] & 0x80000000u) != 0;
+      row[j].add_to(acc);
+      if (!ends && i0 + j + 1 < to) continue;
+      const int64_t id = ids[i0 + j];
+      if (id >= a.vocab) return;  // the ids without a gradient are the last
+      float f[V];
+      Row::get(acc, f);
+      if (ends && !earlier) {
+        write_row<T, V>(a, id, c, f);
+      } else {
+        float *dst = a.part + ((int64_t)chunk * 2 + (earlier ? 0 : 1)) * a.wide + c;
+        if constexpr (V == 8) {
+          store8f(dst, f);
+        } else {
+          dst[0] = f[0];
+        }
+      }
+      earlier = false;
+      Row::clear(acc);
+    }
+  }
+}
+
 // CTAs [0, chunks x slices) sum, the others (`fill_ctas`) fill zeros: both only need the sorted keys
 // and write different rows, so the fill hides the sums' latencies and the sums cost their bytes.
-// G: dy's type, T: dW's. V columns a thread (8 on 16-byte aligned rows, else 1); kAhead rows of dy
-// in flight, whatever ids they belong to.
+// G: dy's type, T: dW's. V columns a thread (8 on 16-byte aligned rows, else 1).
 template <int G, int T, int V>
 __global__ void __launch_bounds__(kSumThreads) sum_chunks(SumArgs a, int chunks, int sums) {
   pdl_wait();
@@ -340,7 +383,6 @@ __global__ void __launch_bounds__(kSumThreads) sum_chunks(SumArgs a, int chunks,
     fill_rows(a, (int)a.hidden * elem_size<T>(), before, (int)fill);
     return;
   }
-  constexpr int kAhead = 8;
   const int me = (int)blockIdx.x - before, slice = me / chunks, chunk = me - slice * chunks;
   // of the chunk's places: the token, with bit 31 set where its id ends; the id
   __shared__ uint32_t sh_tok[kMaxChunk];
@@ -360,40 +402,7 @@ __global__ void __launch_bounds__(kSumThreads) sum_chunks(SumArgs a, int chunks,
   __syncthreads();
   const int64_t c = ((int64_t)slice * blockDim.x + threadIdx.x) * V;
   if (c >= a.hidden) return;
-  using Row = RawRow<G, V>;
-  typename Row::Sum acc;
-  Row::clear(acc);
-  bool earlier = sh_earlier;
-  for (int i0 = 0; i0 < count; i0 += kAhead) {
-    Row row[kAhead];
-    const int m = count - i0;
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j)
-      if (j < m) row[j].load(a.dy, (int64_t)(sh_tok[i0 + j] & 0x7fffffffu) * a.hidden + c);
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      if (j >= m) break;
-      const bool ends = (sh_tok[i0 + j] & 0x80000000u) != 0;
-      row[j].add_to(acc);
-      if (!ends && i0 + j + 1 < count) continue;
-      const int64_t id = sh_id[i0 + j];
-      if (id >= a.vocab) return;  // the ids without a gradient are the last
-      float f[V];
-      Row::get(acc, f);
-      if (ends && !earlier) {
-        write_row<T, V>(a, id, c, f);
-      } else {
-        float *dst = a.part + ((int64_t)chunk * 2 + (earlier ? 0 : 1)) * a.wide + c;
-        if constexpr (V == 8) {
-          store8f(dst, f);
-        } else {
-          dst[0] = f[0];
-        }
-      }
-      earlier = false;
-      Row::clear(acc);
-    }
-  }
+  sum_places<G, T, V>(a, sh_tok, sh_id, 0, count, sh_earlier, chunk, c);
 }
 
 // Adds partials i0, i0 + step, ... of `count` to s (partial 0 is the second row of chunk `first`,
@@ -486,6 +495,81 @@ __global__ void __launch_bounds__(kSumThreads, 4) join_chunks(SumArgs a, int64_t
     }
     __syncthreads();
   }
+}
+
+// Up to kSmall tokens in one launch, without a workspace: every CTA sorts the keys for itself (2 us),
+// then sums the ids that begin in its places, whole, or fills zeros.
+template <int G, int T, int V>
+__global__ void __launch_bounds__(kSmall)
+    grad_small(SumArgs a, const void *__restrict__ ids, bool ids64, int64_t pad, int chunks,
+               int sums) {
+  pdl_wait();
+  pdl_release();
+  __shared__ uint64_t buf[2][kSmall];
+  __shared__ uint32_t sh_tok[kSmall], sh_id[kSmall], sh_starts[kSmall / 32];
+  __shared__ uint8_t used[kFillRows];
+  const int t = threadIdx.x, lane = t & 31, n = (int)a.n;
+  uint64_t k = 0xffffffffull << 32 | (uint32_t)t;
+  if (t < n)
+    k = (uint64_t)(ids64 ? sort_id(static_cast<const int64_t *>(ids), t, a.vocab, pad)
+                         : sort_id(static_cast<const int32_t *>(ids), t, a.vocab, pad)) << 32 |
+        (uint32_t)t;
+#pragma unroll
+  for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+    for (int stride = size / 2; stride > 0; stride /= 2) k = lane_step(k, lane, size, stride);
+  int from = 0;
+  buf[0][t] = k;
+  __syncthreads();
+  for (int run = 32; run < n; run *= 2) {
+    const uint64_t *other = buf[from] + ((t / run) ^ 1) * run;
+    int place = 0;
+    k = buf[from][t];
+    for (int half = run; half > 0; half /= 2)
+      if (place + half <= run && other[place + half - 1] < k) place += half;
+    buf[from ^ 1][t / (2 * run) * (2 * run) + t % run + place] = k;
+    __syncthreads();
+    from ^= 1;
+  }
+  k = buf[from][t];
+  const uint32_t id = (uint32_t)(k >> 32);
+  const bool ends = t + 1 >= n || (uint32_t)(buf[from][t + 1] >> 32) != id;
+  const bool starts = t >= n || t == 0 || (uint32_t)(buf[from][t - 1] >> 32) != id;
+  sh_tok[t] = (uint32_t)k | (ends ? 0x80000000u : 0u);
+  sh_id[t] = id;
+  const uint32_t word = __ballot_sync(0xffffffffu, starts);
+  if (lane == 0) sh_starts[t / 32] = word;
+  __syncthreads();
+  const int64_t fill = (int64_t)gridDim.x - sums;
+  const int before = (int)(fill * blockIdx.x / gridDim.x);
+  if ((int)(fill * (blockIdx.x + 1) / gridDim.x) != before) {
+    const int64_t row_bytes = a.hidden * elem_size<T>();
+    for (int64_t r0 = (int64_t)before * kFillRows; r0 < a.vocab; r0 += fill * kFillRows) {
+      const int count = (int)(a.vocab - r0 < kFillRows ? a.vocab - r0 : kFillRows);
+      if (t < kFillRows) used[t] = 0;
+      __syncthreads();
+      if (t < n && (int64_t)id >= r0 && (int64_t)id < r0 + count) used[id - r0] = 1;
+      __syncthreads();
+      for (int i = t / 32; i < count; i += kSmall / 32)
+        if (!used[i]) warp_zero(static_cast<uint8_t *>(a.dw) + (r0 + i) * row_bytes, row_bytes);
+      __syncthreads();
+    }
+    return;
+  }
+  const int me = (int)blockIdx.x - before, slice = me / chunks, chunk = me - slice * chunks;
+  const int64_t c = ((int64_t)slice * kSmall + t) * V;
+  if (c >= a.hidden) return;
+  // the first start at or behind a place (n behind the last)
+  auto start_from = [&](int p) {
+    for (int w = p / 32; w < kSmall / 32; ++w) {
+      const uint32_t bits = sh_starts[w] & (w == p / 32 ? 0xffffffffu << (p % 32) : 0xffffffffu);
+      if (bits) return w * 32 + __ffs(bits) - 1;
+    }
+    return kSmall;
+  };
+  const int s = start_from(chunk * a.chunk);
+  const int e = (chunk + 1) * a.chunk < n ? start_from((chunk + 1) * a.chunk) : n;
+  if (s < n) sum_places<G, T, V>(a, sh_tok, sh_id, s, e < n ? e : n, false, 0, c);
 }
 
 // Vectors of V columns, numbered through the tokens (`cols` to a token), kAhead in flight a thread;
@@ -593,6 +677,27 @@ GradPlan grad_plan(int64_t n, int64_t hidden) {
   return p;
 }
 
+template <int G, int T>
+int run_small(SumArgs a, const void *ids, bool ids64, int64_t pad, cudaStream_t st) {
+  const bool vec = a.hidden % 8 == 0 && aligned(a.dy, 16) && aligned(a.dw, 16);
+  const int64_t slices = ((vec ? a.hidden / 8 : a.hidden) + kSmall - 1) / kSmall;
+  a.chunk = a.n > 64 ? 4 : 1;
+  const int chunks = (int)((a.n + a.chunk - 1) / a.chunk);
+  int64_t fill = 0;
+  if (!a.accumulate) {
+    fill = (int64_t)sm_count() * 4;
+    const int64_t units = (a.vocab + kFillRows - 1) / kFillRows;
+    if (fill > units) fill = units;
+  }
+  const int64_t sums = chunks * slices;
+  const dim3 grid((unsigned)(sums + fill));
+  if (vec)
+    return launch("embedding_grad", grad_small<G, T, 8>, grid, kSmall, 0, st, a, ids, ids64, pad,
+                  chunks, (int)sums);
+  return launch("embedding_grad", grad_small<G, T, 1>, grid, kSmall, 0, st, a, ids, ids64, pad,
+                chunks, (int)sums);
+}
+
 template <typename I>
 int run_sort(const I *ids, int64_t n, int64_t vocab, int64_t pad, uint64_t *keys, int64_t tiles,
              const Early &early, cudaStream_t st) {
@@ -680,7 +785,7 @@ extern "C" int tb_embedding_fwd(const void *ids, int32_t ids_int64, const void *
 }
 
 extern "C" int64_t tb_embedding_grad_workspace(int64_t n, int64_t hidden) {
-  if (n <= 0 || hidden <= 0) return 0;
+  if (n <= kSmall || hidden <= 0) return 0;
   const GradPlan p = grad_plan(n, hidden);
   return 2 * p.keys_bytes + p.part_bytes;
 }
@@ -702,11 +807,23 @@ extern "C" int tb_embedding_grad(const void *ids, int32_t ids_int64, const void 
   if (!aligned(dw, es) || !aligned(dy, elem_size_of(dy_type)) || !aligned(ids, ids_int64 ? 8 : 4) ||
       !aligned(workspace, 16))
     return set_error(TB_EALIGN, "embedding_grad: a buffer is not aligned to its element");
-  if (n > 0 && (!workspace || workspace_bytes < tb_embedding_grad_workspace(n, hidden)))
+  if (n > kSmall && (!workspace || workspace_bytes < tb_embedding_grad_workspace(n, hidden)))
     return set_error(TB_EINVAL, "embedding_grad: workspace of %lld bytes, %lld needed",
                      (long long)workspace_bytes,
                      (long long)tb_embedding_grad_workspace(n, hidden));
   cudaStream_t st = as_stream(stream);
+#define TB_WITH_GRAD(RUN)                                            \
+  do {                                                               \
+    if (dy_type == type) TB_WITH_TYPE(type, T, RUN(T, T));           \
+    if (dy_type == TB_FP32) TB_WITH_TYPE(type, T, RUN(TB_FP32, T));  \
+    TB_WITH_TYPE(dy_type, G, RUN(G, TB_FP32));                       \
+  } while (0)
+  if (n <= kSmall) {
+    const SumArgs a{nullptr, dy, dw, nullptr, n, hidden, vocab, hidden, 0, 1, scale, accumulate != 0};
+#define TB_SMALL(G, T) return run_small<G, T>(a, ids, ids_int64 != 0, padding_idx, st)
+    TB_WITH_GRAD(TB_SMALL);
+#undef TB_SMALL
+  }
   const GradPlan p = grad_plan(n, hidden);
   uint8_t *ws = static_cast<uint8_t *>(workspace);
   uint64_t *keys = reinterpret_cast<uint64_t *>(ws);
@@ -720,7 +837,7 @@ extern "C" int tb_embedding_grad(const void *ids, int32_t ids_int64, const void 
     if (!accumulate) cleared = cleared + bytes / row_bytes < vocab ? cleared + bytes / row_bytes : vocab;
     early.hi = cleared * row_bytes;
   };
-  if (n > 0) {
+  {
     clear_rows(kSortClears);
     rc = ids_int64
              ? run_sort(static_cast<const int64_t *>(ids), n, vocab, padding_idx, keys, p.tiles, early,
@@ -746,8 +863,7 @@ extern "C" int tb_embedding_grad(const void *ids, int32_t ids_int64, const void 
   const SumArgs a{keys,  dy,    dw,      reinterpret_cast<float *>(ws + 2 * p.keys_bytes),
                   n,     hidden, vocab, p.wide, cleared, p.chunk, scale, accumulate != 0};
 #define TB_SUM(G, T) return run_sums<G, T>(a, p.chunks, st)
-  if (dy_type == type) TB_WITH_TYPE(type, T, TB_SUM(T, T));
-  if (dy_type == TB_FP32) TB_WITH_TYPE(type, T, TB_SUM(TB_FP32, T));
-  TB_WITH_TYPE(dy_type, G, TB_SUM(G, TB_FP32));
+  TB_WITH_GRAD(TB_SUM);
 #undef TB_SUM
+#undef TB_WITH_GRAD
 }

@@ -15,6 +15,9 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 
 
+SMALL = 256  # tokens whose gradient takes one launch and no workspace
+
+
 def _check_ids(ids, what):
     if ids.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"{what}: ids must be int64 or int32, got {ids.dtype}")
@@ -23,12 +26,13 @@ def _check_ids(ids, what):
 
 def _grad(ids, dy, dw, scale, padding_idx, accumulate):
     n, (vocab, hidden) = ids.numel(), dw.shape
-    nbytes = _lib.workspace_bytes(dw, "tb_embedding_grad_workspace", n, hidden)
-    ws = dw.new_empty(max(nbytes, 16), dtype=torch.uint8)
+    # no workspace up to SMALL tokens (and no call to ask for it)
+    nbytes = 0 if n <= SMALL else _lib.load().tb_embedding_grad_workspace(n, hidden)
+    ws = dw.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     _lib.call_on(dw, "tb_embedding_grad", ids.data_ptr(), int(ids.dtype == torch.int64),
                  dy.data_ptr(), _lib.TYPE_CODES[dy.dtype], dw.data_ptr(),
                  _lib.TYPE_CODES[dw.dtype], scale, padding_idx, int(accumulate), n, hidden, vocab,
-                 ws.data_ptr(), nbytes)
+                 _lib.addr(ws), nbytes)
     return dw
 
 
