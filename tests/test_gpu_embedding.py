@@ -112,6 +112,7 @@ def test_added_to_an_existing_gradient(dtype, dy_dtype, hidden):
     out = old.clone().to(DEV)
     assert embedding_grad(ids.to(DEV), dy.to(DEV), 900, scale=0.5, out=out) is out
     _check_grad(out, ids, dy, 900, 0.5, old=old)
+    assert out._version > 0
     empty = embedding_grad(ids[:0].to(DEV), dy[:0].to(DEV), 900, out=out)
     assert empty is out
 

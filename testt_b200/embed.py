@@ -117,5 +117,8 @@ def embedding_grad(ids, dy, vocab, scale=1.0, padding_idx=None, out=None, dtype=
             raise ValueError(f"embedding_grad: operands on {t.device} and {dy.device}")
     accumulate = out is not None
     dw = out if accumulate else torch.empty((vocab, hidden), dtype=dtype, device=dy.device)
-    return _grad(ids, dy.contiguous(), dw, float(scale),
-                 -1 if padding_idx is None else int(padding_idx), accumulate)
+    _grad(ids, dy.contiguous(), dw, float(scale), -1 if padding_idx is None else int(padding_idx),
+          accumulate)
+    if accumulate:
+        torch.autograd.graph.increment_version(out)  # autograd sees the write
+    return dw
