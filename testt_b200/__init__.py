@@ -12,6 +12,13 @@ of include/testt_b200.h:
 - nf4.py      NF4 unpacking (plain and double-quant) for every frozen projection
 - model.py    the Qwen2 training forward on real (non-pad) tokens built from the above
 - dist.py     data-parallel LoRA gradient all-reduce and the vocab-sharded head merge
+
+and, for steps that path does not cover, operators of their own (fp16, bf16, fp32):
+
+- embed.py      scaled embedding with its gradient by sorted tokens
+- norm_rope.py  per-head norms of queries and keys with the rotation
+- logprobs.py   log-probabilities of given tokens, entropy and top alternatives, with gradients
+- dropout.py    dropout from a counter-based generator, no stored mask
 """
 
 __version__ = "0.1.0"
