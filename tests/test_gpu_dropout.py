@@ -154,3 +154,18 @@ def test_refusals():
         dropout(x.cpu(), 0.1, 0)
     assert dropout(x[:0], 0.1, 0).numel() == 0
     assert np.array_equal(dropout(x[:0].reshape(0, 4), 0.1, 0).shape, (0, 4))
+
+
+def test_offsets_past_32_bits():
+    """More than 2^32 elements: the last ones draw the words of their own numbers."""
+    from testt_b200.dropout import dropout
+
+    if torch.cuda.mem_get_info()[0] < 40e9:
+        pytest.skip("needs 40 GB of device memory")
+    n = 2 ** 32 + 1003
+    x = torch.ones(n, dtype=torch.float16, device=DEV)
+    y = dropout(x, 0.5, 21, 5)
+    first = n - 1003
+    words = rowops.philox_words(21, 5 + first // 4, 1003)
+    assert np.array_equal((y[first:] != 0).cpu().numpy(), words >= np.uint64(2 ** 31))
+    assert torch.equal(y[:1000].cpu() != 0, rowops.keep_mask((1000,), 0.5, 21, 5))

@@ -221,3 +221,28 @@ def test_refusals():
             bad()
     with pytest.raises(RuntimeError, match="CUDA tensors"):
         embedding(ids.cpu(), w)
+
+
+def test_offsets_past_32_bits():
+    """A table and a gradient of more than 2^31 elements: rows at their far end."""
+    from testt_b200.embed import embedding
+
+    if torch.cuda.mem_get_info()[0] < 24e9:
+        pytest.skip("needs 24 GB of device memory")
+    vocab, hidden = 140001, 16384
+    table = torch.zeros(vocab, hidden, dtype=torch.float16, device=DEV).requires_grad_()
+    rows = torch.randn(3, hidden, device=DEV).half()
+    ids = torch.tensor([vocab - 1, 131072, 5, vocab - 1], device=DEV)
+    with torch.no_grad():
+        table[ids[:3]] = rows
+    y = embedding(ids, table, scale=2.0)
+    assert torch.equal(y, (rows * 2)[[0, 1, 2, 0]])
+    for copies in (1, 100):  # one launch; the sort, the sums and the join
+        many = ids.repeat(copies)
+        dy = torch.ones(many.numel(), hidden, dtype=torch.float16, device=DEV)
+        (dw,) = torch.autograd.grad(embedding(many, table, scale=2.0), table, dy)
+        sums = dw.sum(1, dtype=torch.float32)
+        want = torch.zeros(vocab, device=DEV)
+        want.index_add_(0, ids, torch.full((4,), 2.0 * copies * hidden, device=DEV))
+        assert torch.equal(sums, want)
+        del dw

@@ -219,3 +219,36 @@ def test_refusals_and_empty():
     assert q.shape == (0, 4, 64)
     dqkv, dqw = torch.autograd.grad(q.sum() + v.sum(), [e["qkv"], e["q_weight"]])
     assert dqkv.shape == e["qkv"].shape and torch.all(dqw == 0)
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 elements of q|k|v, outputs and gradient: the last tokens equal the same
+    tokens alone."""
+    from testt_b200.norm_rope import norm_rope_tokens
+
+    if torch.cuda.mem_get_info()[0] < 40e9:
+        pytest.skip("needs 40 GB of device memory")
+    rows, nh, nkv, d = 280001, 48, 8, 128
+    g = torch.Generator().manual_seed(3)
+    tail = torch.randn(5, (nh + 2 * nkv) * d, generator=g).half().to(DEV)
+    cos, sin = torch.randn(2, 16, d, generator=g).to(DEV)
+    w = torch.rand(d, generator=g).half().to(DEV)
+    qkv = torch.zeros(rows, (nh + 2 * nkv) * d, dtype=torch.float16, device=DEV)
+    qkv[-5:] = tail
+    pos = torch.arange(rows, device=DEV) % 16
+    grads = [torch.randn(5, h, d, generator=g).half().to(DEV) for h in (nh, nkv, nkv)]
+
+    def run(x, at, weight):
+        x, weight = x.requires_grad_(), weight.clone().requires_grad_()
+        outs = norm_rope_tokens(x, None, None, weight, None, 1e-6, cos, sin, at, 1, 16, nh, nkv, d)
+        full = [torch.zeros_like(o) for o in outs]
+        for f, t in zip(full, grads):
+            f[-5:] = t
+        return outs, torch.autograd.grad(outs, [x, weight], full)
+
+    outs, (dx, dw) = run(qkv, pos, w)
+    alone, (dx5, dw5) = run(tail, pos[-5:], w)
+    for a, b in zip(outs, alone):
+        assert torch.equal(a[-5:], b) and not a[:-5].any()
+    assert torch.equal(dx[-5:], dx5) and not dx[:-5].any()
+    assert torch.allclose(dw.float(), dw5.float(), rtol=2.0 ** -9)
