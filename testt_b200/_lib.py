@@ -7,6 +7,7 @@ surrounding PyTorch work.
 """
 
 import ctypes
+import functools
 import os
 
 import torch
@@ -142,7 +143,7 @@ def call(name, *args):
     """Calls entry point `name`; raises KernelError with the library's message on failure."""
     global _calls
     _calls += 1
-    rc = getattr(load(), name)(*args)
+    rc = getattr(_lib or load(), name)(*args)
     if rc != 0:
         msg = load().tb_last_error().decode(errors="replace")
         raise KernelError(f"{name} failed ({rc}): {msg}")
@@ -160,13 +161,15 @@ def call_on(t, name, *args):
     return call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(index, name, *args):
+    with torch.cuda.device(index):
+        return getattr(load(), name)(*args)
+
+
 def workspace_bytes(t, name, *args):
-    """A workspace size (which may depend on the device) with the tensor's device current."""
-    index = t.get_device()
-    if index != torch._C._cuda_getDevice():
-        with torch.cuda.device(index):
-            return getattr(load(), name)(*args)
-    return getattr(load(), name)(*args)
+    """A workspace size, which depends on the sizes given and on the tensor's device (asked once)."""
+    return _workspace_bytes(t.get_device(), name, *args)
 
 
 def addr(t):

@@ -15,19 +15,15 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 
 
-SMALL = 256  # tokens whose gradient takes one launch and no workspace
-
-
 def _check_ids(ids, what):
     if ids.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"{what}: ids must be int64 or int32, got {ids.dtype}")
-    return ids.contiguous()
+    return ids if ids.is_contiguous() else ids.contiguous()
 
 
 def _grad(ids, dy, dw, scale, padding_idx, accumulate):
     n, (vocab, hidden) = ids.numel(), dw.shape
-    # no workspace up to SMALL tokens (and no call to ask for it)
-    nbytes = 0 if n <= SMALL else _lib.load().tb_embedding_grad_workspace(n, hidden)
+    nbytes = _lib.workspace_bytes(dw, "tb_embedding_grad_workspace", n, hidden)
     ws = dw.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     _lib.call_on(dw, "tb_embedding_grad", ids.data_ptr(), int(ids.dtype == torch.int64),
                  dy.data_ptr(), _lib.TYPE_CODES[dy.dtype], dw.data_ptr(),
@@ -72,7 +68,7 @@ def embedding(ids, weight, scale=1.0, padding_idx=None, out_dtype=None):
     if weight.dtype not in _lib.TYPE_CODES or weight.dim() != 2 or 0 in weight.shape:
         raise ValueError(f"embedding: weight must be fp16, bf16 or fp32 [vocab, hidden], got "
                          f"{tuple(weight.shape)} {weight.dtype}")
-    if ids.device != weight.device:
+    if ids.get_device() != weight.get_device():
         raise ValueError(f"embedding: ids on {ids.device}, weight on {weight.device}")
     out_dtype = weight.dtype if out_dtype is None else out_dtype
     if out_dtype not in (weight.dtype, torch.float32):

@@ -107,7 +107,7 @@ def token_logprobs(logits, ids, top_k=0, temperature=1.0):
     if ids.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"token_logprobs: ids must be int64 or int32, got {ids.dtype}")
     lead, vocab = logits.shape[:-1], logits.shape[-1]
-    if ids.shape != lead or ids.device != logits.device:
+    if ids.shape != lead or ids.get_device() != logits.get_device():
         raise ValueError(f"token_logprobs: ids {tuple(ids.shape)} on {ids.device} for logits "
                          f"{tuple(logits.shape)} on {logits.device}")
     top_k = int(top_k)
