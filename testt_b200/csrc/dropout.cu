@@ -7,8 +7,8 @@
 // selected away, not multiplied by 0, so an infinity or NaN that is dropped leaves nothing.
 //
 // 33.6 M elements: fp16 x + fp32 residual -> fp32 50 us (336 MB, the memory's rate), the backward
-// fp32 -> fp16 41 us (202 MB, 31 us at that rate): 80 integer issue slots per four elements then
-// weigh as much as the bytes. Persistent CTAs with the next vector in flight took 55 / 46 us.
+// fp32 -> fp16 41 us (202 MB, 31 us at that rate): the generator's integer work then weighs as much
+// as the bytes (issue 63 %, DRAM 48 %). Persistent CTAs with the next vector in flight took 55 / 46 us.
 //
 // Reference: solution/model.py:195-206 runs PyTorch's dropout, which stores a byte mask.
 #include "dtypes.cuh"

@@ -4,17 +4,23 @@
 //   gradient   dW[v] = scale * sum over the tokens t with id_t = v of dy[t]   (0 without tokens)
 //
 // The gradient sorts the keys (id << 32 | t), all different, so the order does not depend on
-// timing: tiles of kTile keys by a bitonic network in shared memory, then groups of kWays sorted
+// timing: tiles of kTile keys in shared memory (see sort_tiles), then groups of kWays sorted
 // runs are merged by ranks (a key's place in the merged run is its place in its own run plus the
 // number of smaller keys in each other run, found by bisection). The tokens of one id are then
 // neighbours. A CTA of the sum kernel takes kChunk places of the sorted order and all columns of
 // a slice, adds rows in fp32 while the id stays, and writes an id's row when it ends. An id that
 // crosses chunks leaves one fp32 partial row per chunk, which the join kernel adds in the order of
 // the chunks. So each dy row is read once, each dW row is rounded once and no float atomics run.
-// Rows of ids without tokens are zeros. The sum launch writes them too, with CTAs of their own that
-// look the ids with tokens up in the sorted keys: they are most of the dense gradient's bytes
+// Rows of ids without tokens are zeros. The sort's launches clear the first of them with idle CTAs,
+// the sum launch writes the rest with CTAs that look the ids with tokens up in the sorted keys: they are most of the dense gradient's bytes
 // ([151936, 1536] fp16 is 467 MB, against 621 tokens' 2 MB). With accumulate set nothing is zeroed
 // and the sums are added to what dW holds.
+//
+// Measured, in us (sum of the launches' device times; DRAM as a share of the nominal rate):
+//   621 tokens, [151936, 1536] fp16: forward 3.4, gradient 84 (sort 12, sums and zeros 68, join 4),
+//     bound by the 467 MB it writes (71 at the rate of a copy).
+//   32749 tokens, [50021, 2056] bf16: forward 33 (42 % of DRAM), gradient 102 (sort 14, merge 24, sums
+//     and zeros 51 at 61 % of DRAM, join 13), bound by the sort's and the gathers' latencies.
 //
 // Reference: solution/model.py:220-225 embeds the real tokens with a frozen table.
 #include "dtypes.cuh"
