@@ -151,6 +151,54 @@ def test_nan_and_infinity_stay_in_their_row(bad):
     assert torch.isnan(o.top_logprobs).all() and int(o.top_ids.max()) < 100
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("temp", [1.0, 1e-4, 1e4])
+@pytest.mark.parametrize("rows", [3, 700])
+def test_spreads_past_fp32(dtype, temp, rows):
+    """Logits whose differences, or whose differences over the temperature, are no fp32 numbers:
+    those far below the largest have probability 0 and leave no NaN."""
+    from testt_b200.logprobs import token_logprobs
+
+    vocab, k = 2500, 3
+    logits = _logits(rows, vocab, dtype, 8, std=1e37)
+    logits[:, 7], logits[:, 2049], logits[:, 1300] = -3e38, 3e38, 1e38
+    logits[1] = _logits(1, vocab, dtype, 9, std=1e12)[0]
+    ids = torch.tensor([7, 2049, 1300]).repeat(rows)[:rows]
+    z = logits.to(DEV).requires_grad_()
+    o = token_logprobs(z, ids.to(DEV), top_k=k, temperature=temp)
+    g = torch.Generator().manual_seed(3)
+    grads = [torch.randn(rows, generator=g), torch.randn(rows, generator=g),
+             torch.randn(rows, k, generator=g)]
+    w = rowops.token_logprobs(logits, ids, k, temp, grads)
+    as_fp32 = lambda t: t.float().double()  # noqa: E731  (-inf past its range)
+    tol = _sum_tol(vocab)
+    fin = lambda t: torch.nan_to_num(t.abs(), posinf=0.0)  # noqa: E731
+    # the difference, 1 / T, the products and the sum with log S round: 6 U of it
+    assert_rounded(o.logprob, as_fp32(w["lp"]), tol + 6 * U * fin(as_fp32(w["lp"])), "lp")
+    assert_rounded(o.top_logprobs, as_fp32(w["top_lp"]), tol + 6 * U * fin(as_fp32(w["top_lp"])),
+                   "top")
+    assert torch.equal(o.top_ids.cpu(), w["top_ids"])
+    assert_rounded(o.entropy, w["ent"], (2 * tol + 8 * U) * (1 + math.log(vocab)), "entropy")
+    (dz,) = torch.autograd.grad([o.logprob, o.entropy, o.top_logprobs], z, [t.to(DEV) for t in grads])
+    # the spreads leave one logit of probability 1 or gaps of at least 1e5 U below it (1e12 / 1e4)
+    ge = grads[1].double().abs()[:, None]
+    d = torch.where(w["p"] > 0, w["p"].clamp_min(1e-300).log2().abs(), torch.zeros_like(w["p"]))
+    extra = w["dz_mag"] * (tol + (4 * d + 16 + k) * U) + \
+        w["p"] * ge * (2 * tol + 8 * U) * (1 + math.log(vocab)) / temp + 2.0 ** -126 / temp * (1 + ge)
+    assert_rounded(dz, w["dz"], extra, "dz")
+
+
+@pytest.mark.parametrize("rows", [2, 700])
+def test_nan_among_minus_infinities(rows):
+    from testt_b200.logprobs import token_logprobs
+
+    z = torch.full((rows, 900), -math.inf)
+    z[0, 333] = math.nan
+    o = token_logprobs(z.to(DEV), torch.zeros(rows, dtype=torch.long, device=DEV), top_k=2)
+    for t in (o.logprob, o.top_logprobs[:, 0]):
+        assert torch.isnan(t[0]) and torch.isneginf(t[1:]).all()
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("a,b", [(0, 1001), (3, 1004), (8, 1009), (5, 9)])
 def test_rows_of_a_wider_buffer(dtype, a, b):

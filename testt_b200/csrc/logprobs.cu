@@ -5,7 +5,7 @@
 //   d logits = (1/T) (g_lp (1_id - p) + sum_j g_j (1_top_j - p) - g_H p (log p + H))
 //
 // Forward: an online softmax per thread over the raw logits x: a running maximum m, t = x - m,
-// S = sum 2^(t c) with c = log2(e) / T, U = sum 2^(t c) t; lp = ln2 (t_id c - log2 S) and
+// S = sum 2^(t c) with c = log2(e) / T, U = sum 2^(t c) t; lp = t_id / T - ln2 log2 S and
 // H = ln2 log2 S - U / (S T). Differences, not products, are taken first, so logits of any size
 // keep their precision. Logits count as kLow = -1e20 at least inside the sums, so a -inf mask (or
 // the type's lowest value) adds 2^.. = 0 and 0 * t stays 0; max.NaN keeps a NaN, which makes the
@@ -40,6 +40,7 @@ constexpr int kUnroll = 4;       // 16-byte vectors in flight per thread
 constexpr int kAgain = 2;        // vectors in flight per thread when they are read again
 constexpr int kMaxTop = 32;      // one list entry per lane
 constexpr float kLow = -1e20f;   // logits below it count as it
+constexpr float kFar = -1e25f;   // exponents are held at it where they are factors: 2^kFar is 0
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr uint32_t kAll = 0xffffffffu;
@@ -254,7 +255,7 @@ struct Running {
   __device__ __forceinline__ void one(float x, float c) {  // x below m already
     const float d = (max_nan(x, kLow) - ref) * c, p = ex2(d);
     s += p;
-    u = fmaf(p, d, u);
+    u = fmaf(p, fmaxf(d, kFar), u);
   }
 };
 
@@ -277,11 +278,14 @@ __device__ __forceinline__ int64_t id_of(const void *ids, bool ids64, int64_t ro
                : (int64_t)static_cast<const int32_t *>(ids)[row];
 }
 
-// Log-probability of logit x in a row of state a, l = log2 S.
-__device__ __forceinline__ float logprob_of(float x, const State &a, float l, float c,
-                                            float inv_t) {
-  if (x < kLow) return a.m == -CUDART_INF_F ? x : (x - a.m) * inv_t - kLn2 * l;
-  return kLn2 * fmaf(x - reference(a.m), c, -l);
+// Log-probability of logit x in a row of state a, l = log2 S. Logits below kLow keep their own value
+// here. The difference is halved where it may be past fp32 although its product with 1 / T is not.
+__device__ __forceinline__ float logprob_of(float x, const State &a, float l, float inv_t) {
+  if (a.m == -CUDART_INF_F) return l == l ? x : l;  // no logit above -inf, perhaps a NaN
+  const float ref = x < kLow ? a.m : reference(a.m);
+  float d = (x - ref) * inv_t;
+  if (d == -CUDART_INF_F) d = 2.f * ((0.5f * x - 0.5f * ref) * inv_t);
+  return d - kLn2 * l;
 }
 
 // The row's given id and its logit (0 for an id outside).
@@ -296,7 +300,7 @@ __device__ __forceinline__ void finish_row(const FwdArgs &a, int64_t row, const 
   const float l = log2f(st.s);
   const bool empty = st.m == -CUDART_INF_F && st.s == st.s;
   if (lane == 0) {
-    a.logprob[row] = id >= 0 && id < a.vocab ? logprob_of(x, st, l, a.c, a.inv_t) : 0.f;
+    a.logprob[row] = id >= 0 && id < a.vocab ? logprob_of(x, st, l, a.inv_t) : 0.f;
     float h = kLn2 * (l - st.u / st.s);
     h = empty || h < 0.f ? 0.f : h;
     a.entropy[row] = h;
@@ -307,7 +311,7 @@ __device__ __forceinline__ void finish_row(const FwdArgs &a, int64_t row, const 
   if (lane < a.k) {
     a.top_ids[row * a.k + lane] = key == 0 ? 0 : (int64_t)key_index(key);
     a.top_lp[row * a.k + lane] =
-        key == 0 ? CUDART_NAN_F : logprob_of(key_value(key), st, l, a.c, a.inv_t);
+        key == 0 ? CUDART_NAN_F : logprob_of(key_value(key), st, l, a.inv_t);
   }
 }
 
@@ -398,7 +402,7 @@ __device__ __forceinline__ void add_batch(Running<T> &r, uint4 (&raw)[N], float 
       for (int e = 0; e < E; ++e) {
         const float d = (max_nan(z[e], kLow) - r.ref) * c, p = ex2(d);
         s += p;
-        u = fmaf(p, d, u);
+        u = fmaf(p, fmaxf(d, kFar), u);  // d may be past fp32: 0 times it is no NaN
       }
     }
   }
@@ -562,7 +566,7 @@ struct BwdArgs {
 // p (G + g_H (log p + H)) of a logit: d = log2 p, A and B hold the factors.
 __device__ __forceinline__ float slope(float x, float ref, float l, float c, float A, float B) {
   const float d = fmaf(max_nan(x, kLow) - ref, c, -l);
-  return ex2(d) * fmaf(B, d, A);
+  return ex2(d) * fmaf(B, fmaxf(d, kFar), A);
 }
 
 template <int T>
