@@ -114,6 +114,35 @@ def test_no_key_value_heads_and_missing_gradients():
     assert torch.all(dkw == 0)
 
 
+@pytest.mark.parametrize("n,nkv", [(1, 2), (5, 0), (1, 0)])
+def test_gradients_share_no_memory(n, nkv):
+    """The LoRA rows' gradients are qkv's columns: where those are whole, autograd keeps what it is
+    given, and a later change of one leaf's gradient must not reach another's."""
+    from testt_b200.norm_rope import norm_rope_tokens
+
+    c, grads = _case(n, 4, nkv, 64, 64, 8, torch.float32, torch.float32, torch.float32, seed=15)
+    g = _gpu(c)
+    leaves = [g[x].requires_grad_() for x in ("qkv", "lora_q", "lora_v")]
+    out = norm_rope_tokens(**g)
+    torch.autograd.backward(out, [t.to(DEV) for t in grads])
+    want = [t.grad.clone() for t in leaves]
+    for i, t in enumerate(leaves):
+        t.grad.add_(1.0)
+        want[i] += 1.0
+        for u, v in zip(leaves, want):
+            assert torch.equal(u.grad, v)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d", [64, 20])
+def test_small_heads_without_eps(dtype, d):
+    """Heads of 1e-14 with eps 0: 1 / rms is 1e14, whose cube is no fp32 number."""
+    c, grads = _case(9, 4, 2, d, d, 8, dtype, weights=dtype, seed=16)
+    c["qkv"] = (c["qkv"].float() * 1e-14).to(dtype)
+    c["eps"] = 0.0
+    _check(c, grads)
+
+
 def test_only_values_used():
     from testt_b200.norm_rope import norm_rope_tokens
 

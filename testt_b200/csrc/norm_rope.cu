@@ -552,7 +552,8 @@ __global__ void __launch_bounds__(kThreads, kBwdPerSm)
           gx = group_sum(gx, sp.lanes);
           const float r = rsqrtf(fmaf(ss, dm.inv_d, dm.eps));
           if (live && inside) {
-            const F2 rr = both(r), rk = both(-(r * r * r) * gx * dm.inv_d);
+            // r gx first: r^3 alone may be past fp32
+            const F2 rr = both(r), rk = both(-(r * gx * dm.inv_d) * r * r);
 #pragma unroll
             for (int i = 0; i < V / 4; ++i) {
 #pragma unroll
