@@ -605,8 +605,8 @@ int tb_embedding_fwd(const void *ids, int32_t ids_int64, const void *table, int3
  * tokens, contiguous [vocab, hidden] in `type`; with `accumulate` the sums are added to what dw
  * holds and rows of other ids are left alone. Ids outside [0, vocab) and `padding_idx` (-1: none)
  * give nothing. fp32 sums in a fixed order (the tokens sorted by id, then position), rounded once.
- * dy [n, hidden] in `type`, or TB_FP32, or any type when `type` is TB_FP32. `workspace`:
- * tb_embedding_grad_workspace bytes, 16-byte aligned. */
+ * dy [n, hidden] in `type`, or TB_FP32, or any type when `type` is TB_FP32. n is at most 2^31 - 2^16
+ * here and above. `workspace`: tb_embedding_grad_workspace bytes, 16-byte aligned. */
 int tb_embedding_grad(const void *ids, int32_t ids_int64, const void *dy, int32_t dy_type, void *dw,
                       int32_t type, float scale, int64_t padding_idx, int32_t accumulate,
                       int64_t n, int64_t hidden, int64_t vocab, void *workspace,

@@ -82,6 +82,15 @@ def test_embedding(lib):
         _refuses(lib, "tb_embedding_grad", grad[:i] + [v] + grad[i + 1:], code, text)
 
 
+def test_embedding_token_limit(lib):
+    """More tokens than a launch's grid can merge are refused before any launch."""
+    n = 0x7fff0001
+    for name, args in (("tb_embedding_fwd", [P(256), 1, P(256), 0, 64, P(256), 2, 1.0, n, 64, 100, None]),
+                       ("tb_embedding_grad", [P(256), 1, P(256), 0, P(256), 0, 1.0, -1, 0, n, 64, 100,
+                                              P(256), 2 ** 62, None])):
+        _refuses(lib, name, args, TB_EINVAL, b"n 2147418113")
+
+
 def test_token_logprobs(lib):
     need = lib.tb_token_logprobs_workspace(4, 100000, 0, 4)  # few long rows are split
     assert need > 0 and lib.tb_token_logprobs_workspace(0, 100000, 0, 4) == 0

@@ -38,6 +38,7 @@ constexpr int kSmall = 256;         // tokens the one-launch gradient takes
 constexpr int kFillRows = 32;       // ids whose zero rows a CTA looks for at a time
 constexpr int64_t kSortClears = 40 << 20, kMergeClears = 64 << 20;  // bytes cleared meanwhile
 constexpr int kMaxChunk = 32;       // places of the sorted order a CTA sums
+constexpr int64_t kMaxTokens = 0x7fff0000;  // whose merge groups, one more with the clearing, a grid's y holds
 constexpr uint64_t kNoKey = ~0ull;  // padding of the last tile
 
 __device__ unsigned int g_invalid = 0;
@@ -746,7 +747,7 @@ int run_sums(const SumArgs &a, int64_t chunks, cudaStream_t st) {
 }
 
 int check_sizes(const char *what, int64_t n, int64_t hidden, int64_t vocab) {
-  if (n < 0 || hidden <= 0 || vocab <= 0 || n > 0x7fffffffLL || vocab > 0x7fffffffLL ||
+  if (n < 0 || hidden <= 0 || vocab <= 0 || n > kMaxTokens || vocab > 0x7fffffffLL ||
       hidden > (1 << 20))
     return set_error(TB_EINVAL, "%s: n %lld hidden %lld vocab %lld", what, (long long)n,
                      (long long)hidden, (long long)vocab);
