@@ -633,7 +633,7 @@ int tb_token_logprobs_fwd(const void *logits, int32_t type, int64_t ld, const vo
 /* Its gradient: grad [rows, vocab] in `type`, rows ld_grad apart, for the gradients of logprob,
  * entropy and top_logprobs (each may be NULL: zero): (1/T) (g_lp (1_id - p) + sum_j g_top_j
  * (1_top_j - p) - g_H p (log p + H)); zero on rows of -inf only. grad's rows must lie modulo 16
- * bytes as the logits' rows do (TB_EALIGN otherwise). */
+ * bytes as the logits' rows do (TB_EALIGN otherwise), and are not the logits' own memory. */
 int tb_token_logprobs_bwd(const void *logits, int32_t type, int64_t ld, const void *ids,
                           int32_t ids_int64, float temperature, int32_t top_k,
                           const int64_t *top_ids, const float *stats, const float *g_logprob,

@@ -91,6 +91,13 @@ def test_embedding_token_limit(lib):
         _refuses(lib, name, args, TB_EINVAL, b"n 2147418113")
 
 
+def test_token_logprobs_gradient_is_not_the_logits(lib):
+    """The columns with a one-hot term are read again after the row is written."""
+    args = [P(256), 0, 1000, P(256), 1, 1.0, 0, None, P(256), P(256), None, None, P(256), 1000, 4,
+            1000, None]
+    _refuses(lib, "tb_token_logprobs_bwd", args, TB_EINVAL, b"the logits themselves")
+
+
 def test_token_logprobs(lib):
     need = lib.tb_token_logprobs_workspace(4, 100000, 0, 4)  # few long rows are split
     assert need > 0 and lib.tb_token_logprobs_workspace(0, 100000, 0, 4) == 0

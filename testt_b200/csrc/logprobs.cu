@@ -748,6 +748,8 @@ extern "C" int tb_token_logprobs_bwd(const void *logits, int32_t type, int64_t l
       (rows > 1 && (ld - ld_grad) * es % 16 != 0))
     return set_error(TB_EALIGN, "token_logprobs_bwd: the gradient's rows must lie modulo 16 bytes "
                                 "as the logits' rows do");
+  if (grad == logits)  // the columns with a one-hot term are read again after the row is written
+    return set_error(TB_EINVAL, "token_logprobs_bwd: grad is the logits themselves");
   const int64_t nv = most_vecs(vocab, es);
   const int64_t per = (int64_t)kThreads * kUnroll * 4;
   int64_t splits = (nv + per - 1) / per;
