@@ -18,13 +18,14 @@
 // all differ and settle ties by the lowest index, in descending lists over a warp's lanes.
 //
 // Measured (6.55 TB/s is a plain copy's rate):
-//   2048 x 151936 bf16, top 5: forward 125 us (622 MB, 5.0 TB/s), backward 197 us (1245 MB, 6.3 TB/s)
-//   1531 x 50021 fp32, top 8: 71 us (306 MB, 4.3 TB/s) and 92 us (613 MB, 6.6 TB/s)
-//   621 x 151936 fp16: 44 us (189 MB, 4.3 TB/s; 4.2 rows an SM) and 60 us (377 MB, 6.3 TB/s)
-// The backward is bound by memory; the 16-bit forward by the exponentials (their pipe is 65 % busy at
-// 621 rows) and by each row's CTA start and reductions, about 2 us a row an SM. Reading the next batch
-// of vectors ahead costs registers or L1 and lost (57 against 48 us by registers; by a ring of copies
-// 135 against 125 at 2048 rows).
+//   2048 x 151936 bf16, top 5: forward 125 us (622 MB, 5.0 TB/s), backward 187 us (1245 MB, 6.7 TB/s)
+//   1531 x 50021 fp32, top 8: 71 us (306 MB, 4.3 TB/s) and 90 us (613 MB, 6.8 TB/s)
+//   621 x 151936 fp16: 44 us (189 MB, 4.3 TB/s; 4.2 rows an SM) and 56 us (377 MB, 6.8 TB/s)
+// The backward is bound by memory; no unit is full in the forward, whose CTAs wait for their vectors,
+// then compute, then reduce (about 2 us a row an SM). Reading the next batch of vectors ahead costs
+// registers or L1 and lost (57 against 48 us by registers; by a ring of copies 135 against 125 at 2048
+// rows), and so did an eighth of the exponentials by a polynomial (129; their pipe is 65 % busy at 621
+// rows).
 //
 // Beside the head's statistics over given logits (solution/head.py:34-76, tb_head_stats_grad).
 #include <math_constants.h>
@@ -36,7 +37,12 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kUnroll = 4;       // 16-byte vectors in flight per thread
+// 16-byte vectors in flight per thread of the forward, at five CTAs an SM (2048 x 151936 bf16: 124 us;
+// 2 at eight CTAs 138, 3 at six 135, 6 at four 128, 8 at three 132).
+constexpr int kUnroll = 4;
+// Of the backward, and batches a CTA takes. 621 x 151936 fp16 / 2048 x 151936 bf16, in us: 2 vectors by 4
+// batches 56 / 187, by 2 62 / 208, by 16 58 / 195; 4 by 4 59 / 193; 1 by 8 63 / 188.
+constexpr int kBwdUnroll = 2, kBwdBatches = 4;
 constexpr int kAgain = 2;        // vectors in flight per thread when they are read again
 constexpr int kMaxTop = 32;      // one list entry per lane
 constexpr float kLow = -1e20f;   // logits below it count as it
@@ -622,11 +628,11 @@ __global__ void __launch_bounds__(kThreads) logprobs_bwd(BwdArgs a) {
   const uint4 *vecs = reinterpret_cast<const uint4 *>(r.base + r.head * elem_size<T>());
   uint4 *out_vecs = reinterpret_cast<uint4 *>(out + r.head * elem_size<T>());
   int64_t v = v0 + threadIdx.x;
-  for (; v + (kUnroll - 1) * kThreads < v1; v += kUnroll * kThreads) {
-    uint4 raw[kUnroll];
+  for (; v + (kBwdUnroll - 1) * kThreads < v1; v += kBwdUnroll * kThreads) {
+    uint4 raw[kBwdUnroll];
     load_batch(vecs + v, raw);
 #pragma unroll
-    for (int b = 0; b < kUnroll; ++b)
+    for (int b = 0; b < kBwdUnroll; ++b)
       out_vecs[v + b * kThreads] = slopes<T>(raw[b], ref, l, a.c, A, B);
   }
   for (; v < v1; v += kThreads) out_vecs[v] = slopes<T>(__ldg(vecs + v), ref, l, a.c, A, B);
@@ -751,7 +757,7 @@ extern "C" int tb_token_logprobs_bwd(const void *logits, int32_t type, int64_t l
   if (grad == logits)  // the columns with a one-hot term are read again after the row is written
     return set_error(TB_EINVAL, "token_logprobs_bwd: grad is the logits themselves");
   const int64_t nv = most_vecs(vocab, es);
-  const int64_t per = (int64_t)kThreads * kUnroll * 4;
+  const int64_t per = (int64_t)kThreads * kBwdUnroll * kBwdBatches;
   int64_t splits = (nv + per - 1) / per;
   if (splits > 1024) splits = 1024;
   const BwdArgs a{logits, ids, top_ids, stats, g_logprob, g_entropy, g_top, grad, rows,
