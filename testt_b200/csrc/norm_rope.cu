@@ -10,8 +10,8 @@
 // the lanes, then (a second kernel) of the CTAs, so results do not depend on timing.
 //
 // 16411 tokens of 32 + 8 + 8 heads of 128, half of each turned, bf16: forward 82 us (403 MB, 4.9
-// TB/s), backward 135 + 3 us (571 MB, 4.2 TB/s); a plain copy runs at 6.55 TB/s. Bound by issue and
-// shared-memory reads at 16 to 24 warps an SM, not by DRAM: one CTA a token with everything in
+// TB/s), backward 131 + 3 us (571 MB, 4.4 TB/s); a plain copy runs at 6.55 TB/s. Bound by fixed and
+// shared-memory latencies at 24 and 16 warps an SM, not by DRAM: one CTA a token with everything in
 // registers took 259 / 291 us (one CTA an SM), deeper rings change nothing. Packed fp32 pairs halve
 // the arithmetic's issue slots; the rotation's factors lie in shared memory once a warp and token,
 // as 32 registers less a lane allow half as many warps again.
