@@ -11,6 +11,7 @@ import functools
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 # TESTT_B200_LIB points at another build of the same library (for example a debug build)
@@ -178,12 +179,24 @@ def addr(t):
 
 
 def needs_grad(*tensors):
-    """Whether autograd would record a call on these tensors."""
+    """Whether autograd has to see a call on these tensors: it would record it, or a forward-mode
+    level is open, in which a tensor's tangent shows in no flag of its own (a call that goes through
+    an autograd.Function then raises NotImplementedError instead of dropping it)."""
+    if forward_ad._current_level >= 0:
+        return True
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 return True
     return False
+
+
+def refuse_tangents(what, *tensors):
+    """Raises for tensors with a forward-mode tangent that a call on raw pointers would drop."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{what}: no forward-mode derivative")
 
 
 def launch_count():

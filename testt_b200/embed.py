@@ -87,7 +87,8 @@ def embedding_grad(ids, dy, vocab, scale=1.0, padding_idx=None, out=None, dtype=
     """embedding's weight gradient [vocab, hidden] for dy [*ids.shape, hidden], in `dtype` (dy's by
     default; dy's, or either of the two fp32). With `out` (contiguous, its dtype such a one) the
     sums are added to it in place, each touched row rounded once more, and it is returned: the
-    form for a table tied to the head, whose gradient holds the head's share already."""
+    form for a table tied to the head, whose gradient holds the head's share already. Not
+    differentiable itself: dy and out are taken as values."""
     _lib.require_cuda(ids, dy, out, what="embedding_grad")
     ids = _check_ids(ids, "embedding_grad")
     if dy.dtype not in _lib.TYPE_CODES or dy.dim() != ids.dim() + 1 or \
@@ -111,6 +112,7 @@ def embedding_grad(ids, dy, vocab, scale=1.0, padding_idx=None, out=None, dtype=
     for t in (ids, out):
         if t is not None and t.device != dy.device:
             raise ValueError(f"embedding_grad: operands on {t.device} and {dy.device}")
+    _lib.refuse_tangents("embedding_grad", dy, out)
     accumulate = out is not None
     dw = out if accumulate else torch.empty((vocab, hidden), dtype=dtype, device=dy.device)
     _grad(ids, dy.contiguous(), dw, float(scale), -1 if padding_idx is None else int(padding_idx),
