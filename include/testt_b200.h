@@ -620,8 +620,8 @@ int64_t tb_embedding_grad_workspace(int64_t n, int64_t hidden);
  * in `type`, rows ld elements apart; ids (int64, or int32 when ids_int64 is 0): logprob[r] =
  * log softmax(logits[r] / temperature)[ids[r]], 0 where ids[r] is outside [0, vocab); entropy[r];
  * top_logprobs / top_ids [rows, top_k] (top_k 0 to 32): the largest, equal ones by the lowest
- * index. stats fp32 [rows, 3] is what the backward needs. Logits below -1e20 count as -1e20 in the
- * row's sum. A row of -inf only gives logprob -inf and entropy 0; a NaN or +inf makes its row's
+ * index. stats fp32 [rows, 3] is what the backward needs. A -inf logit has probability 0 beside
+ * any finite one. A row of -inf only gives logprob -inf and entropy 0; a NaN or +inf makes its row's
  * results NaN (top_ids in range). Temperature 1e-4 to 1e4, rows below 2^21. `workspace`:
  * tb_token_logprobs_workspace bytes, 16-byte aligned. */
 int tb_token_logprobs_fwd(const void *logits, int32_t type, int64_t ld, const void *ids,

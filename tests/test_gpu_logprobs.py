@@ -131,6 +131,51 @@ def test_masks(dtype, rows):
     assert o.logprob[1] == 0 and o.entropy[1] == 0
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("temp", [1.0, 1e-4, 1e4])
+@pytest.mark.parametrize("rows", [5, 700])
+def test_lowest_values_beside_minus_infinities(dtype, temp, rows):
+    """Rows whose largest logit is the type's lowest value or lies far below the usual ones, with
+    -inf columns beside it: those have probability 0 and no gradient, the finite ones their own
+    differences. Columns 0 to 2 and the last ones lie outside the whole 16-byte vectors of some rows."""
+    v = 5003
+    low = torch.finfo(dtype).min
+    z = torch.full((rows, v), -math.inf)
+    z[:, :3] = low
+    z[1::5, 100:4000] = low
+    z[2::5, v - 1] = low
+    z[3::5, 50:3000] = low / 2
+    z[3::5, 60:70] = low / 4
+    z[4::5, 7:v:2] = -3e4 if dtype == torch.float16 else -2e20
+    ids = _ids(rows, v)
+    ids[:2] = torch.tensor([1, 4500])  # a finite logit, a -inf one
+    ids[3::5] = 65
+    z = z.to(dtype)
+    o, dz = _check(z, ids, 3, temp)
+    zero = torch.isneginf(z)
+    zero[torch.arange(rows)[ids >= 0], ids[ids >= 0]] = False
+    assert torch.all(dz.cpu()[zero] == 0)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_large_gradients_of_masked_rows(dtype):
+    """Masked columns add nothing to a gradient of any size: powers of two times the incoming
+    gradients give that times the outgoing one, bit for bit (no probability here is near the smallest
+    normal number)."""
+    from testt_b200.logprobs import token_logprobs
+
+    z = _logits(5, 2000, dtype, 12)
+    z[:, 1500:] = -math.inf
+    z[2, ::3] = torch.finfo(dtype).min
+    z = z.to(DEV).requires_grad_()
+    o = token_logprobs(z, _ids(5, 1500).to(DEV), temperature=0.7)
+    gs = torch.randn(2, 5, device=DEV)
+    (small,) = torch.autograd.grad(o[:2], z, list(gs), retain_graph=True)
+    for e in (20, 66, 100):
+        (big,) = torch.autograd.grad(o[:2], z, list(gs * 2.0 ** e), retain_graph=True)
+        assert torch.equal(big.double(), small.double() * 2.0 ** e)
+
+
 @pytest.mark.parametrize("bad", [math.nan, math.inf])
 def test_nan_and_infinity_stay_in_their_row(bad):
     from testt_b200.logprobs import token_logprobs

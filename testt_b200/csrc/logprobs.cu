@@ -7,9 +7,10 @@
 // Forward: an online softmax per thread over the raw logits x: a running maximum m, t = x - m,
 // S = sum 2^(t c) with c = log2(e) / T, U = sum 2^(t c) t; lp = t_id / T - ln2 log2 S and
 // H = ln2 log2 S - U / (S T). Differences, not products, are taken first, so logits of any size
-// keep their precision. Logits count as kLow = -1e20 at least inside the sums, so a -inf mask (or
-// the type's lowest value) adds 2^.. = 0 and 0 * t stays 0; max.NaN keeps a NaN, which makes the
-// row's results NaN. A row of -inf only has lp -inf, entropy 0 and no gradient.
+// keep their precision. m counts as -FLT_MAX at least there, so t is never -inf - -inf: a -inf mask
+// adds 2^-inf = 0 beside any finite logits, the type's lowest value included, and exponents are held
+// at kFar where they are factors, so that 0 * t stays 0. A NaN makes the row's results NaN. A row of
+// -inf only has S = 0, lp -inf, entropy 0 and no gradient.
 //
 // Top k without work per logit: every thread knows its own maximum (the softmax needs it anyway).
 // The k-th largest of the threads' maxima is a lower bound of the row's k-th largest logit, and
@@ -45,8 +46,9 @@ constexpr int kUnroll = 4;
 constexpr int kBwdUnroll = 2, kBwdBatches = 4;
 constexpr int kAgain = 2;        // vectors in flight per thread when they are read again
 constexpr int kMaxTop = 32;      // one list entry per lane
-constexpr float kLow = -1e20f;   // logits below it count as it
-constexpr float kFar = -1e25f;   // exponents are held at it where they are factors: 2^kFar is 0
+// Logits are held at it where the sums' reference is known to be above -1e12: 2^.. is 0 for both.
+constexpr float kLow = -1e20f;
+constexpr float kFar = -1024.f;  // exponents are held at it where they are factors: 2^kFar is 0
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr uint32_t kAll = 0xffffffffu;
@@ -199,11 +201,11 @@ __device__ __forceinline__ void warp_insert(uint64_t &list, uint64_t key, int k,
   }
 }
 
-struct State {  // max, and S and U about max(max, kLow)
+struct State {  // max, and S and U about max(max, -FLT_MAX)
   float m, s, u;
 };
 
-__device__ __forceinline__ float reference(float m) { return fmaxf(m, kLow); }
+__device__ __forceinline__ float reference(float m) { return fmaxf(m, -CUDART_MAX_NORMAL_F); }
 
 // (s, u) about m moved to a reference m2 >= m.
 __device__ __forceinline__ void move_to(float &s, float &u, float m, float m2, float c) {
@@ -259,7 +261,7 @@ struct Running {
     u += bu;
   }
   __device__ __forceinline__ void one(float x, float c) {  // x below m already
-    const float d = (max_nan(x, kLow) - ref) * c, p = ex2(d);
+    const float d = (x - ref) * c, p = ex2(d);
     s += p;
     u = fmaf(p, fmaxf(d, kFar), u);
   }
@@ -284,13 +286,12 @@ __device__ __forceinline__ int64_t id_of(const void *ids, bool ids64, int64_t ro
                : (int64_t)static_cast<const int32_t *>(ids)[row];
 }
 
-// Log-probability of logit x in a row of state a, l = log2 S. Logits below kLow keep their own value
-// here. The difference is halved where it may be past fp32 although its product with 1 / T is not.
+// Log-probability of logit x in a row of state a, l = log2 S. The difference is halved where it may
+// be past fp32 although its product with 1 / T is not.
 __device__ __forceinline__ float logprob_of(float x, const State &a, float l, float inv_t) {
   if (a.m == -CUDART_INF_F) return l == l ? x : l;  // no logit above -inf, perhaps a NaN
-  const float ref = x < kLow ? a.m : reference(a.m);
-  float d = (x - ref) * inv_t;
-  if (d == -CUDART_INF_F) d = 2.f * ((0.5f * x - 0.5f * ref) * inv_t);
+  float d = (x - a.m) * inv_t;
+  if (d == -CUDART_INF_F) d = 2.f * ((0.5f * x - 0.5f * a.m) * inv_t);
   return d - kLn2 * l;
 }
 
@@ -406,7 +407,7 @@ __device__ __forceinline__ void add_batch(Running<T> &r, uint4 (&raw)[N], float 
       unpack_vec<T>(raw[b], z);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const float d = (max_nan(z[e], kLow) - r.ref) * c, p = ex2(d);
+        const float d = (z[e] - r.ref) * c, p = ex2(d);
         s += p;
         u = fmaf(p, fmaxf(d, kFar), u);  // d may be past fp32: 0 times it is no NaN
       }
@@ -571,7 +572,7 @@ struct BwdArgs {
 
 // p (G + g_H (log p + H)) of a logit: d = log2 p, A and B hold the factors.
 __device__ __forceinline__ float slope(float x, float ref, float l, float c, float A, float B) {
-  const float d = fmaf(max_nan(x, kLow) - ref, c, -l);
+  const float d = fmaf(x - ref, c, -l);
   return ex2(d) * fmaf(B, fmaxf(d, kFar), A);
 }
 

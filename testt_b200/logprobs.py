@@ -98,10 +98,9 @@ def token_logprobs(logits, ids, top_k=0, temperature=1.0):
     """TokenLogprobs of fp16, bf16 or fp32 `logits` [..., vocab] (unit column stride is taken as it
     is, rows may be views) at int64 or int32 `ids` [...]; `top_k` 0 to 32. Differentiable in the
     logits through logprob, entropy and top_logprobs. An id outside [0, vocab) (IGNORE_INDEX) has
-    logprob 0 and no gradient; -inf logits have probability 0; logits below -1e20 count as -1e20 in
-    the row's sum (a row of the type's lowest value is one of equal logits); a row of -inf only has
-    logprob -inf, entropy 0 and no gradient; a NaN or +inf makes its row NaN. Fewer than 2^21
-    rows."""
+    logprob 0 and no gradient; -inf logits have probability 0, beside the type's lowest value too (a
+    row of that value is one of equal logits); a row of -inf only has logprob -inf, entropy 0 and no
+    gradient; a NaN or +inf makes its row NaN. Fewer than 2^21 rows."""
     _lib.require_cuda(logits, ids, what="token_logprobs")
     if logits.dtype not in _lib.TYPE_CODES or logits.dim() < 1 or logits.shape[-1] == 0:
         raise ValueError(f"token_logprobs: logits must be fp16, bf16 or fp32 [..., vocab], got "
