@@ -99,6 +99,26 @@ def test_rows_of_a_wider_buffer(width, start):
     _check(c, grads, gpu=g)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d,rot", [(64, 64), (80, 40), (20, 20), (20, 6)])
+def test_several_tokens_a_warp(d, rot, dtype):
+    """As many tokens as make every warp of every kernel walk on from one to the next (at most 3,552
+    and 18,944 warps forward, 2,368 and 1,184 backward on 148 SMs), on tables whose halves differ,
+    with LoRA rows, weights and positions outside."""
+    n, nh, nkv = 9001, 2, 1
+    c, grads = _case(n, nh, nkv, d, rot, 700, dtype, torch.float32 if d == 64 else dtype, dtype,
+                     seed=17, outside=True)
+    c["pos_idx"][5::97] = 2 * 700
+    g = torch.Generator().manual_seed(18)
+    c["cos"], c["sin"] = torch.randn(2, 700, rot, generator=g)
+    got = _check(c, grads, w0=0.5)[3]
+    want = _oracle(c, 0.5, grads)
+    # a weight's sum: at most 8 tokens of 2 heads in a lane, 64 lanes' sums, 37 CTAs', 32 groups'
+    for name in "qk":
+        assert_rounded(got[name + "_weight"], want[f"d{name}w"],
+                       want[f"d{name}w_mag"] * (16 + 64 + 37 + 32 + d + 32) * U, name + "_weight")
+
+
 def test_no_key_value_heads_and_missing_gradients():
     from testt_b200.norm_rope import norm_rope_tokens
 
