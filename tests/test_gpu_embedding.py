@@ -64,6 +64,46 @@ def test_forward_and_gradient(n, vocab, hidden, kind, dtype):
         _check_grad(dw, ids, dy, vocab, scale, what="dw")
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,hidden", [(1301, 4104), (701, 1001)])
+def test_forward_of_many_vectors(n, hidden, dtype):
+    """More vectors (of 8 columns, of one) than the persistent forward has threads for at a time
+    (606,208 on 148 SMs), with ids outside."""
+    from testt_b200 import _lib
+    from testt_b200.embed import embedding
+
+    vocab = 2000
+    ids = _ids(n, vocab, n, "uniform")
+    ids[::50], ids[7::300] = vocab, -5
+    outside = int(((ids < 0) | (ids >= vocab)).sum())
+    table = _table(vocab, hidden, dtype, 14)
+    want = rowops.embedding(ids, table, 3.3)
+    for out, index in ((dtype, torch.int64), (torch.float32, torch.int32)):
+        before = _lib.load().tb_embed_invalid_ids()
+        y = embedding(ids.to(DEV, index), table.to(DEV), scale=3.3, out_dtype=out)
+        assert_rounded(y, want, want.abs() * 2 * U, "y")
+        assert _lib.load().tb_embed_invalid_ids() == before + outside
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [2 ** 21 - 2, 2 ** 21 - 1, 2 ** 22 + 77])
+@pytest.mark.parametrize("hidden", [8, 3])
+def test_large_vocabularies(vocab, hidden, dtype):
+    """Vocabularies around the one from which on a tile's keys take 64 bits: ids that differ in
+    their high bits alone, repeated, the last ones, the padding id and ids outside."""
+    from testt_b200.embed import embedding_grad
+
+    n = 4500
+    ids = _ids(n, vocab, 15)
+    ids[::3] = torch.randint(0, 7, (n // 3,), generator=torch.Generator().manual_seed(16)) \
+        + 2 ** 20 * torch.arange(n // 3).remainder(2)
+    ids[1::9], ids[2::90], ids[4::90] = vocab - 1, vocab, -1
+    ids[5::30] = vocab - 2 - torch.arange(n // 30).remainder(3)
+    dy = torch.randn(n, hidden, generator=torch.Generator().manual_seed(17)).to(dtype)
+    got = embedding_grad(ids.to(DEV), dy.to(DEV), vocab, scale=1.5, padding_idx=2)
+    _check_grad(got, ids, dy, vocab, 1.5, pad=2)
+
+
 @pytest.mark.parametrize("n,kind", [(33000, "zipf"), (33000, "same"), (70001, "uniform")])
 def test_many_tiles_merge(n, kind):
     """More tokens than one merge takes (16 tiles of 2048), ids over many chunks."""
