@@ -568,8 +568,12 @@ int tb_dropout(const void *x, int32_t x_type, const void *residual, void *y, int
  * (weight_offset + weight) (a NULL weight: 1), turned on their first `rot` dims by row
  * pos_idx[token] % seq of cos / sin (fp32 [seq, rot]); v = x. q [rows, n_heads, head_dim], k and
  * v [rows, n_kv, head_dim] in `type`. A token whose position is outside [0, batch * seq) gives
- * zero rows. head_dim (at most 4096) and rot even; multiples of 8 up to 256 with buffers aligned to
- * four elements (tables to 16 bytes) take the vector path. */
+ * zero rows. head_dim (at most 4096) and rot even. The vector path takes
+ *   16-bit types with head_dim (up to 512) and rot multiples of 16, where every row of qkv, q, k and
+ *   v starts on 16 bytes; other multiples of 8 (head_dim up to 256), where it starts on 8;
+ *   fp32 with head_dim (up to 256) and rot multiples of 8, where it starts on 16;
+ * each with the LoRA rows, weights and tables on 16 bytes, LoRA rows and weights in `type` or
+ * TB_FP32. Anything else takes a path for any size, several times slower. */
 int tb_norm_rope_fwd(const void *qkv, int32_t type, int64_t ld, const void *lora_q,
                      const void *lora_v, int32_t lora_type, const void *q_weight,
                      const void *k_weight, int32_t weight_type, float weight_offset, float eps,
@@ -581,7 +585,8 @@ int tb_norm_rope_fwd(const void *qkv, int32_t type, int64_t ld, const void *lora
  * head_dim] contiguous, from dq, dk, dv (each may be NULL: zero) and the forward's inputs; and,
  * when dq_weight / dk_weight are given, the weights' gradients (weight_type), whose fp32 sums over
  * token ranges go to `workspace` (tb_norm_rope_bwd_workspace bytes) and are added in a fixed
- * order. Outside positions give zero rows. */
+ * order. Outside positions give zero rows. The paths are chosen as in the forward, by the rows of dq,
+ * dk, dv and dqkv too. */
 int tb_norm_rope_bwd(const void *dq, const void *dk, const void *dv, const void *qkv, int32_t type,
                      int64_t ld, const void *lora_q, int32_t lora_type, const void *q_weight,
                      const void *k_weight, int32_t weight_type, float weight_offset, float eps,

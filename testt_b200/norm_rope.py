@@ -104,7 +104,10 @@ def norm_rope_tokens(qkv, lora_q, lora_v, q_weight, k_weight, eps, cos, sin, pos
     n_kv * head_dim] are added in fp32 (None: none); `q_weight`, `k_weight` [head_dim] (None: 1);
     `cos`, `sin` [>= seq, rot] with rot <= head_dim; a token's table row is pos_idx % seq, and one
     whose pos_idx is outside [0, batch * seq) gets zero rows and no gradient. qkv's rows may be
-    views of wider rows. Differentiable in qkv, lora_q, lora_v, q_weight and k_weight."""
+    views of wider rows; in 16-bit types rows that do not start on 16 bytes are several times slower
+    than a contiguous copy. Differentiable in qkv, lora_q, lora_v, q_weight and k_weight. Gradients of
+    the LoRA rows are qkv's gradient's columns, as in rope.rope_tokens: fp32 rows beside 16-bit qkv get
+    values rounded to qkv's type (beside fp16, 0 below 3e-8 and infinite above 65504)."""
     _lib.require_cuda(qkv, lora_q, lora_v, q_weight, k_weight, cos, sin, pos_idx,
                       what="norm_rope_tokens")
     dtype, rows = qkv.dtype, qkv.shape[0] if qkv.dim() else 0
