@@ -569,8 +569,8 @@ int tb_dropout(const void *x, int32_t x_type, const void *residual, void *y, int
  * pos_idx[token] % seq of cos / sin (fp32 [seq, rot]); v = x. q [rows, n_heads, head_dim], k and
  * v [rows, n_kv, head_dim] in `type`. A token whose position is outside [0, batch * seq) gives
  * zero rows. head_dim (at most 4096) and rot even. The vector path takes
- *   16-bit types with head_dim (up to 512) and rot multiples of 16, where every row of qkv, q, k and
- *   v starts on 16 bytes; other multiples of 8 (head_dim up to 256), where it starts on 8;
+ *   16-bit types with head_dim (up to 512) and rot multiples of 16, where every row of qkv, q, k
+ *   and v starts on 16 bytes; other multiples of 8 (head_dim up to 256), where it starts on 8;
  *   fp32 with head_dim (up to 256) and rot multiples of 8, where it starts on 16;
  * each with the LoRA rows, weights and tables on 16 bytes, LoRA rows and weights in `type` or
  * TB_FP32. Anything else takes a path for any size, several times slower. */
@@ -585,8 +585,8 @@ int tb_norm_rope_fwd(const void *qkv, int32_t type, int64_t ld, const void *lora
  * head_dim] contiguous, from dq, dk, dv (each may be NULL: zero) and the forward's inputs; and,
  * when dq_weight / dk_weight are given, the weights' gradients (weight_type), whose fp32 sums over
  * token ranges go to `workspace` (tb_norm_rope_bwd_workspace bytes) and are added in a fixed
- * order. Outside positions give zero rows. The paths are chosen as in the forward, by the rows of dq,
- * dk, dv and dqkv too. */
+ * order. Outside positions give zero rows. The paths are chosen as in the forward, by the rows of
+ * dq, dk, dv and dqkv too. */
 int tb_norm_rope_bwd(const void *dq, const void *dk, const void *dv, const void *qkv, int32_t type,
                      int64_t ld, const void *lora_q, int32_t lora_type, const void *q_weight,
                      const void *k_weight, int32_t weight_type, float weight_offset, float eps,
@@ -610,8 +610,8 @@ int tb_embedding_fwd(const void *ids, int32_t ids_int64, const void *table, int3
  * tokens, contiguous [vocab, hidden] in `type`; with `accumulate` the sums are added to what dw
  * holds and rows of other ids are left alone. Ids outside [0, vocab) and `padding_idx` (-1: none)
  * give nothing. fp32 sums in a fixed order (the tokens sorted by id, then position), rounded once.
- * dy [n, hidden] in `type`, or TB_FP32, or any type when `type` is TB_FP32. n is at most 2^31 - 2^16
- * here and above. `workspace`: tb_embedding_grad_workspace bytes, 16-byte aligned. */
+ * dy [n, hidden] in `type`, or TB_FP32, or any type when `type` is TB_FP32. n is at most 2^31 -
+ * 2^16 here and above. `workspace`: tb_embedding_grad_workspace bytes, 16-byte aligned. */
 int tb_embedding_grad(const void *ids, int32_t ids_int64, const void *dy, int32_t dy_type, void *dw,
                       int32_t type, float scale, int64_t padding_idx, int32_t accumulate,
                       int64_t n, int64_t hidden, int64_t vocab, void *workspace,
@@ -625,9 +625,9 @@ int64_t tb_embedding_grad_workspace(int64_t n, int64_t hidden);
  * in `type`, rows ld elements apart; ids (int64, or int32 when ids_int64 is 0): logprob[r] =
  * log softmax(logits[r] / temperature)[ids[r]], 0 where ids[r] is outside [0, vocab); entropy[r];
  * top_logprobs / top_ids [rows, top_k] (top_k 0 to 32): the largest, equal ones by the lowest
- * index. stats fp32 [rows, 3] is what the backward needs. A -inf logit has probability 0 beside
- * any finite one. A row of -inf only gives logprob -inf and entropy 0; a NaN or +inf makes its row's
- * results NaN (top_ids in range). Temperature 1e-4 to 1e4, rows below 2^21. `workspace`:
+ * index. stats fp32 [rows, 3] is what the backward needs. A -inf logit has probability 0
+ * beside any finite one. A row of -inf only gives logprob -inf and entropy 0; a NaN or +inf makes
+ * its row's results NaN (top_ids in range). Temperature 1e-4 to 1e4, rows below 2^21. `workspace`:
  * tb_token_logprobs_workspace bytes, 16-byte aligned. */
 int tb_token_logprobs_fwd(const void *logits, int32_t type, int64_t ld, const void *ids,
                           int32_t ids_int64, float temperature, int32_t top_k, float *logprob,

@@ -137,7 +137,7 @@ def test_masks(dtype, rows):
 def test_lowest_values_beside_minus_infinities(dtype, temp, rows):
     """Rows whose largest logit is the type's lowest value or lies far below the usual ones, with
     -inf columns beside it: those have probability 0 and no gradient, the finite ones their own
-    differences. Columns 0 to 2 and the last ones lie outside the whole 16-byte vectors of some rows."""
+    differences. Columns 0 to 2 and the last lie outside the whole 16-byte vectors of some rows."""
     v = 5003
     low = torch.finfo(dtype).min
     z = torch.full((rows, v), -math.inf)
@@ -160,8 +160,8 @@ def test_lowest_values_beside_minus_infinities(dtype, temp, rows):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_large_gradients_of_masked_rows(dtype):
     """Masked columns add nothing to a gradient of any size: powers of two times the incoming
-    gradients give that times the outgoing one, bit for bit (no probability here is near the smallest
-    normal number)."""
+    gradients give that times the outgoing one, bit for bit (no probability here is near the
+    smallest normal number)."""
     from testt_b200.logprobs import token_logprobs
 
     z = _logits(5, 2000, dtype, 12)

@@ -169,7 +169,7 @@ def _workspace_bytes(index, name, *args):
 
 
 def workspace_bytes(t, name, *args):
-    """A workspace size, which depends on the sizes given and on the tensor's device (asked once)."""
+    """A workspace size, which depends on the sizes and the tensor's device alone (asked once)."""
     return _workspace_bytes(t.get_device(), name, *args)
 
 

@@ -92,8 +92,8 @@ __device__ __forceinline__ void store8(void *p, int64_t i, const float (&f)[8]) 
   }
 }
 
-// Two fp32 values in one 64-bit register pair: sm_100's packed fp32 instructions do two multiply-adds
-// in one issue slot (each rounded as the scalar one).
+// Two fp32 values in one 64-bit register pair: sm_100's packed fp32 instructions do two
+// multiply-adds in one issue slot (each rounded as the scalar one).
 struct F2 {
   uint64_t v;
 };

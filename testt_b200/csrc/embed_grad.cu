@@ -12,15 +12,20 @@
 // crosses chunks leaves one fp32 partial row per chunk, which the join kernel adds in the order of
 // the chunks. So each dy row is read once, each dW row is rounded once and no float atomics run.
 // Rows of ids without tokens are zeros. The sort's launches clear the first of them with idle CTAs,
-// the sum launch writes the rest with CTAs that look the ids with tokens up in the sorted keys: they are most of the dense gradient's bytes
-// ([151936, 1536] fp16 is 467 MB, against 621 tokens' 2 MB). With accumulate set nothing is zeroed
-// and the sums are added to what dW holds.
+// the sum launch writes the rest with CTAs that look the ids with tokens up in the sorted keys:
+// they are most of the dense gradient's bytes ([151936, 1536] fp16 is 467 MB, against 621 tokens'
+// 2 MB). With accumulate set nothing is zeroed and the sums are added to what dW holds.
 //
 // Measured, in us (sum of the launches' device times; DRAM as a share of the nominal rate):
 //   621 tokens, [151936, 1536] fp16: forward 3.4, gradient 84 (sort 12, sums and zeros 68, join 4),
 //     bound by the 467 MB it writes (71 at the rate of a copy).
-//   32749 tokens, [50021, 2056] bf16: forward 33 (42 % of DRAM), gradient 102 (sort 14, merge 24, sums
-//     and zeros 51 at 61 % of DRAM, join 13), bound by the sort's and the gathers' latencies.
+//   32749 tokens, [50021, 2056] bf16: forward 33 (42 % of DRAM), gradient 102 (sort 14, merge 24,
+//     sums and zeros 51 at 61 % of DRAM, join 13): no unit is full in any of the four, which wait
+//     for one another; added to an existing gradient 99 (11, 15, 58, 14).
+//   Up to 256 tokens in one launch: [151936, 1536] fp16 76 to 79, bound by its writes; [2048, 512]
+//     4 to 8, and as much when added to an existing gradient: the sort.
+//   Rows not of 8 columns or off 16 bytes take a column a thread: 32749 tokens, [50021, 2052] fp32
+//     forward 135 (91 with 2056 columns; issue 68 %), gradient 185 (159).
 //
 // Reference: solution/model.py:220-225 embeds the real tokens with a frozen table.
 #include "dtypes.cuh"
@@ -30,7 +35,7 @@ namespace {
 
 constexpr int kTile = 2048;         // keys of one shared-memory sort
 constexpr int kSortThreads = 1024;
-constexpr int kFwdPerSm = 4;        // resident CTAs of the forward (5, at 48 registers: 45 against 33 us)
+constexpr int kFwdPerSm = 4;        // resident CTAs of the forward (33 us; 5, at 48 registers: 45)
 constexpr int kWays = 16;           // runs merged per launch
 constexpr int kSample = 64;         // sampled keys of a run in a merge
 constexpr int kSumThreads = 256;
@@ -38,7 +43,8 @@ constexpr int kSmall = 256;         // tokens the one-launch gradient takes
 constexpr int kFillRows = 32;       // ids whose zero rows a CTA looks for at a time
 constexpr int64_t kSortClears = 40 << 20, kMergeClears = 64 << 20;  // bytes cleared meanwhile
 constexpr int kMaxChunk = 32;       // places of the sorted order a CTA sums
-constexpr int64_t kMaxTokens = 0x7fff0000;  // whose merge groups, one more with the clearing, a grid's y holds
+// Tokens whose merge groups, and one more for the clearing, a grid's y holds.
+constexpr int64_t kMaxTokens = 0x7fff0000;
 constexpr uint64_t kNoKey = ~0ull;  // padding of the last tile
 
 __device__ unsigned int g_invalid = 0;
@@ -97,10 +103,10 @@ __device__ __forceinline__ K lane_step(K k, int lane, int size, int stride) {
 }
 
 // A CTA a tile of kTile tokens. Inside a tile the keys are (id, place in the tile): in 32 bits (K =
-// uint32_t) where the vocabulary is below 2^21 - 1, else in 64. Each warp sorts runs of 32 in its lanes,
-// then neighbouring runs are merged by ranks in shared memory (a key's place is its place in its run
-// plus the smaller keys of the other, by bisection). The 66-step bitonic network over 2048 keys took
-// 21 us for any number of tokens.
+// uint32_t) where the vocabulary is below 2^21 - 1, else in 64. Each warp sorts runs of 32 in its
+// lanes, then neighbouring runs are merged by ranks in shared memory (a key's place is its place in
+// its run plus the smaller keys of the other, by bisection). The 66-step bitonic network over 2048
+// keys took 21 us for any number of tokens.
 template <typename I, typename K>
 __global__ void __launch_bounds__(kSortThreads)
     sort_tiles(const I *__restrict__ ids, int64_t n, int64_t vocab, int64_t pad,
@@ -162,11 +168,11 @@ __global__ void __launch_bounds__(kSortThreads)
   }
 }
 
-// Sorted runs of `run` (a power of two) keys of `in` -> runs of run * kWays keys in `out`: kWays lanes
-// to a key, a lane counts the smaller keys of one run by bisection, the first steps over a sample of
-// kSample keys of each run in shared memory (the probes, not the latencies, are the cost: one thread
-// a key over all runs took 44 us for 32749 keys, kWays lanes without the sample 22 us). A CTA takes
-// keys of one group of runs only: group blockIdx.y.
+// Sorted runs of `run` (a power of two) keys of `in` -> runs of run * kWays keys in `out`: kWays
+// lanes to a key, a lane counts the smaller keys of one run by bisection, the first steps over a
+// sample of kSample keys of each run in shared memory (the probes, not the latencies, are the cost:
+// one thread a key over all runs took 44 us for 32749 keys, kWays lanes without the sample 22 us).
+// A CTA takes keys of one group of runs only: group blockIdx.y.
 __global__ void __launch_bounds__(256)
     merge_runs(const uint64_t *__restrict__ in, uint64_t *__restrict__ out, int64_t n,
                int64_t run, int groups, Early early) {
@@ -376,8 +382,8 @@ __device__ __forceinline__ void sum_places(const SumArgs &a, const uint32_t *tok
   }
 }
 
-// CTAs [0, chunks x slices) sum, the others (`fill_ctas`) fill zeros: both only need the sorted keys
-// and write different rows, so the fill hides the sums' latencies and the sums cost their bytes.
+// `sums` CTAs (chunks x slices) sum, the others fill zeros: both only need the sorted keys and
+// write different rows, so the fill hides the sums' latencies and the sums cost their bytes.
 // G: dy's type, T: dW's. V columns a thread (8 on 16-byte aligned rows, else 1).
 template <int G, int T, int V>
 __global__ void __launch_bounds__(kSumThreads) sum_chunks(SumArgs a, int chunks, int sums) {
@@ -504,8 +510,8 @@ __global__ void __launch_bounds__(kSumThreads, 4) join_chunks(SumArgs a, int64_t
   }
 }
 
-// Up to kSmall tokens in one launch, without a workspace: every CTA sorts the keys for itself (2 us),
-// then sums the ids that begin in its places, whole, or fills zeros.
+// Up to kSmall tokens in one launch, without a workspace: every CTA sorts the keys for itself (2
+// us), then sums the ids that begin in its places, whole, or fills zeros.
 template <int G, int T, int V>
 __global__ void __launch_bounds__(kSmall)
     grad_small(SumArgs a, const void *__restrict__ ids, bool ids64, int64_t pad, int chunks,
@@ -637,8 +643,9 @@ int launch_fwd(const I *ids, const void *table, int64_t ld, void *out, int64_t a
   const FastDiv fd((uint32_t)cols);
   const int64_t resident = (int64_t)sm_count() * 8 * 256;
   if (all <= resident)  // a vector a thread when that does not fill the device
-    return launch("embedding_fwd", embedding_fwd<T, O, V, 1, I>, dim3((unsigned)((all + 255) / 256)),
-                  256, 0, st, ids, table, ld, out, (uint32_t)all, fd, hidden, vocab, scale);
+    return launch("embedding_fwd", embedding_fwd<T, O, V, 1, I>,
+                  dim3((unsigned)((all + 255) / 256)), 256, 0, st, ids, table, ld, out,
+                  (uint32_t)all, fd, hidden, vocab, scale);
   int64_t blocks = (all + 1023) / 1024;
   const int64_t cap = (int64_t)sm_count() * kFwdPerSm;
   if (blocks > cap) blocks = cap;
@@ -656,8 +663,8 @@ int run_fwd(const I *ids, const void *table, int64_t ld, void *out, int64_t n, i
   for (int64_t t = 0; t < n; t += most) {
     const int64_t all = (n - t < most ? n - t : most) * cols;
     void *o = static_cast<char *>(out) + t * hidden * elem_size<O>();
-    const int rc = vec ? launch_fwd<T, O, 8>(ids + t, table, ld, o, all, cols, hidden, vocab, scale, st)
-                       : launch_fwd<T, O, 1>(ids + t, table, ld, o, all, cols, hidden, vocab, scale, st);
+    const auto run = vec ? launch_fwd<T, O, 8, I> : launch_fwd<T, O, 1, I>;
+    const int rc = run(ids + t, table, ld, o, all, cols, hidden, vocab, scale, st);
     if (rc != TB_OK) return rc;
   }
   return TB_OK;
@@ -826,7 +833,8 @@ extern "C" int tb_embedding_grad(const void *ids, int32_t ids_int64, const void 
     TB_WITH_TYPE(dy_type, G, RUN(G, TB_FP32));                       \
   } while (0)
   if (n <= kSmall) {
-    const SumArgs a{nullptr, dy, dw, nullptr, n, hidden, vocab, hidden, 0, 1, scale, accumulate != 0};
+    const SumArgs a{nullptr, dy, dw, nullptr, n,     hidden,
+                    vocab,   hidden, 0, 1, scale, accumulate != 0};
 #define TB_SMALL(G, T) return run_small<G, T>(a, ids, ids_int64 != 0, padding_idx, st)
     TB_WITH_GRAD(TB_SMALL);
 #undef TB_SMALL
@@ -841,16 +849,16 @@ extern "C" int tb_embedding_grad(const void *ids, int32_t ids_int64, const void 
   Early early{static_cast<uint8_t *>(dw), 0, 0};
   auto clear_rows = [&](int64_t bytes) {
     early.lo = cleared * row_bytes;
-    if (!accumulate) cleared = cleared + bytes / row_bytes < vocab ? cleared + bytes / row_bytes : vocab;
+    const int64_t next = cleared + bytes / row_bytes;
+    if (!accumulate) cleared = next < vocab ? next : vocab;
     early.hi = cleared * row_bytes;
   };
   {
     clear_rows(kSortClears);
-    rc = ids_int64
-             ? run_sort(static_cast<const int64_t *>(ids), n, vocab, padding_idx, keys, p.tiles, early,
-                        st)
-             : run_sort(static_cast<const int32_t *>(ids), n, vocab, padding_idx, keys, p.tiles, early,
-                        st);
+    rc = ids_int64 ? run_sort(static_cast<const int64_t *>(ids), n, vocab, padding_idx, keys,
+                              p.tiles, early, st)
+                   : run_sort(static_cast<const int32_t *>(ids), n, vocab, padding_idx, keys,
+                              p.tiles, early, st);
     if (rc != TB_OK) return rc;
   }
   for (int64_t run = kTile; run < n; run *= kWays) {

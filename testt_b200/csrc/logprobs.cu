@@ -8,9 +8,9 @@
 // S = sum 2^(t c) with c = log2(e) / T, U = sum 2^(t c) t; lp = t_id / T - ln2 log2 S and
 // H = ln2 log2 S - U / (S T). Differences, not products, are taken first, so logits of any size
 // keep their precision. m counts as -FLT_MAX at least there, so t is never -inf - -inf: a -inf mask
-// adds 2^-inf = 0 beside any finite logits, the type's lowest value included, and exponents are held
-// at kFar where they are factors, so that 0 * t stays 0. A NaN makes the row's results NaN. A row of
-// -inf only has S = 0, lp -inf, entropy 0 and no gradient.
+// adds 2^-inf = 0 beside any finite logits, the type's lowest value included, and exponents are
+// held at kFar where they are factors, so that 0 * t stays 0. A NaN makes the row's results NaN. A
+// row of -inf only has S = 0, lp -inf, entropy 0 and no gradient.
 //
 // Top k without work per logit: every thread knows its own maximum (the softmax needs it anyway).
 // The k-th largest of the threads' maxima is a lower bound of the row's k-th largest logit, and
@@ -19,14 +19,14 @@
 // all differ and settle ties by the lowest index, in descending lists over a warp's lanes.
 //
 // Measured (6.55 TB/s is a plain copy's rate):
-//   2048 x 151936 bf16, top 5: forward 125 us (622 MB, 5.0 TB/s), backward 187 us (1245 MB, 6.7 TB/s)
-//   1531 x 50021 fp32, top 8: 71 us (306 MB, 4.3 TB/s) and 90 us (613 MB, 6.8 TB/s)
-//   621 x 151936 fp16: 44 us (189 MB, 4.3 TB/s; 4.2 rows an SM) and 56 us (377 MB, 6.8 TB/s)
-// The backward is bound by memory; no unit is full in the forward, whose CTAs wait for their vectors,
-// then compute, then reduce (about 2 us a row an SM). Reading the next batch of vectors ahead costs
-// registers or L1 and lost (57 against 48 us by registers; by a ring of copies 135 against 125 at 2048
-// rows), and so did an eighth of the exponentials by a polynomial (129; their pipe is 65 % busy at 621
-// rows).
+//   2048 x 151936 bf16, top 5: forward 125 us (622 MB, 5.0 TB/s), backward 186 us (1245 MB, 6.7)
+//   1531 x 50021 fp32, top 8: 70 us (306 MB, 4.3 TB/s) and 90 us (613 MB, 6.8)
+//   621 x 151936 fp16: 44 us (189 MB, 4.3 TB/s; 4.2 rows an SM) and 55 us (377 MB, 6.9)
+// The backward is bound by memory; no unit is full in the forward, whose CTAs wait for their
+// vectors, then compute, then reduce (about 2 us a row an SM). Reading the next batch of vectors
+// ahead costs registers or L1 and lost (57 against 48 us by registers; by a ring of copies 135
+// against 125 at 2048 rows), and so did an eighth of the exponentials by a polynomial (129; their
+// pipe is 63 % busy at 621 rows). What is not tried: the CTAs of a cluster sharing a row.
 //
 // Beside the head's statistics over given logits (solution/head.py:34-76, tb_head_stats_grad).
 #include <math_constants.h>
@@ -38,11 +38,11 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-// 16-byte vectors in flight per thread of the forward, at five CTAs an SM (2048 x 151936 bf16: 124 us;
-// 2 at eight CTAs 138, 3 at six 135, 6 at four 128, 8 at three 132).
+// 16-byte vectors in flight per thread of the forward, at five CTAs an SM (2048 x 151936 bf16:
+// 124 us; 2 at eight CTAs 138, 3 at six 135, 6 at four 128, 8 at three 132).
 constexpr int kUnroll = 4;
-// Of the backward, and batches a CTA takes. 621 x 151936 fp16 / 2048 x 151936 bf16, in us: 2 vectors by 4
-// batches 56 / 187, by 2 62 / 208, by 16 58 / 195; 4 by 4 59 / 193; 1 by 8 63 / 188.
+// Of the backward, and batches a CTA takes. 621 x 151936 fp16 / 2048 x 151936 bf16, in us: 2
+// vectors by 4 batches 56 / 187, by 2 62 / 208, by 16 58 / 195; 4 by 4 59 / 193; 1 by 8 63 / 188.
 constexpr int kBwdUnroll = 2, kBwdBatches = 4;
 constexpr int kAgain = 2;        // vectors in flight per thread when they are read again
 constexpr int kMaxTop = 32;      // one list entry per lane
@@ -498,8 +498,9 @@ __global__ void __launch_bounds__(kThreads, T == TB_FP32 ? 6 : 5) logprobs_fwd(F
         if (__ballot_sync(kAll, any) == 0) continue;
 #pragma unroll
         for (int e = 0; e < E; ++e)
-          warp_insert(list, any && z[e] >= bar ? make_key(z[e], r.head + (v0 + at[b]) * E + e) : 0, a.k,
-                      lane);
+          warp_insert(list,
+                      any && z[e] >= bar ? make_key(z[e], r.head + (v0 + at[b]) * E + e) : 0,
+                      a.k, lane);
       }
     }
     list = block_merge(list, sh_list, warp, lane);
@@ -702,7 +703,8 @@ extern "C" int tb_token_logprobs_fwd(const void *logits, int32_t type, int64_t l
   int rc = check("token_logprobs_fwd", rows, vocab, ld, type, top_k, temperature);
   if (rc != TB_OK) return rc;
   if (rows == 0) return TB_OK;
-  if (!logits || !ids || !logprob || !entropy || !stats || (top_k > 0 && (!top_logprobs || !top_ids)))
+  if (!logits || !ids || !logprob || !entropy || !stats ||
+      (top_k > 0 && (!top_logprobs || !top_ids)))
     return set_error(TB_EINVAL, "token_logprobs_fwd: a buffer is missing");
   if (!aligned(logits, elem_size_of(type)) || !aligned(ids, ids_int64 ? 8 : 4) ||
       !aligned(logprob, 4) || !aligned(entropy, 4) || !aligned(stats, 4) ||
@@ -728,8 +730,8 @@ extern "C" int tb_token_logprobs_fwd(const void *logits, int32_t type, int64_t l
                               : launch("token_logprobs_fwd", logprobs_fwd<T, false>, grid,
                                        kThreads, 0, st, a);
                if (rc == TB_OK && splits > 1) rc =
-                   launch("token_logprobs_fwd", logprobs_merge<T>, dim3((unsigned)rows), kThreads, 0, st,
-                          a));
+                   launch("token_logprobs_fwd", logprobs_merge<T>, dim3((unsigned)rows), kThreads,
+                          0, st, a));
   return rc;
 }
 
@@ -737,7 +739,8 @@ extern "C" int tb_token_logprobs_bwd(const void *logits, int32_t type, int64_t l
                                      int32_t ids_int64, float temperature, int32_t top_k,
                                      const int64_t *top_ids, const float *stats,
                                      const float *g_logprob, const float *g_entropy,
-                                     const float *g_top, void *grad, int64_t ld_grad, int64_t rows, int64_t vocab, void *stream) {
+                                     const float *g_top, void *grad, int64_t ld_grad, int64_t rows,
+                                     int64_t vocab, void *stream) {
   int rc = check("token_logprobs_bwd", rows, vocab, ld, type, top_k, temperature);
   if (rc != TB_OK) return rc;
   if (rows == 0) return TB_OK;

@@ -10,9 +10,10 @@
 // the lanes, then (a second kernel) of the CTAs, so results do not depend on timing.
 //
 // 16411 tokens of 32 + 8 + 8 heads of 128, half of each turned, bf16: forward 82 us (403 MB, 4.9
-// TB/s), backward 131 + 3 us (571 MB, 4.4 TB/s); a plain copy runs at 6.55 TB/s. Bound by fixed and
-// shared-memory latencies at 24 and 16 warps an SM, not by DRAM: one CTA a token with everything in
-// registers took 259 / 291 us (one CTA an SM), deeper rings change nothing. Packed fp32 pairs halve
+// TB/s), backward 131 + 3 us (571 MB, 4.4 TB/s); a plain copy runs at 6.55 TB/s. No unit is full:
+// the time goes into fixed and shared-memory latencies at 24 and 16 warps an SM. One CTA a token
+// with everything in registers took 259 / 291 us (one CTA an SM), deeper rings change nothing; bulk
+// copies of a token's whole rows are not tried. Packed fp32 pairs halve
 // the arithmetic's issue slots; the rotation's factors lie in shared memory once a warp and token,
 // as 32 registers less a lane allow half as many warps again.
 //
@@ -157,9 +158,9 @@ __device__ __forceinline__ void stage_weights(float *ws, const void *qw, const v
 }
 
 // ---- the walk of the vector kernels ----------------------------------------------------------
-// The rows of the next stages - 1 groups of a warp's walk are on their way into the lane's own slots
-// of shared memory (cp.async: no registers held, and no barrier, since a lane reads only what it
-// copied).
+// The rows of the next stages - 1 groups of a warp's walk are on their way into the lane's own
+// slots of shared memory (cp.async: no registers held, and no barrier, since a lane reads only what
+// it copied).
 
 constexpr int kFwdStages = 3, kBwdStages = 3;
 
@@ -174,7 +175,9 @@ __device__ __forceinline__ void copy_async(void *dst, const void *src) {
                  : "memory");
 }
 
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void copies_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
 
 template <int N>
 __device__ __forceinline__ void copies_wait() {
@@ -228,11 +231,11 @@ struct Ahead {
   }
 };
 
-// A warp's table of a token's rotation in shared memory, four rows of fp32 quads laid out [row][quad]
-// [lane]: all its head rows use the same factors, so a lane reads them where it needs them instead
-// of holding 4 V registers. Forward rows: y1 = r (x1 A + x2 B), y2 = r (x2 C + x1 D) with the
-// weights inside (A = w1 c1, B = -w2 s1, C = w2 c2, D = w1 s2); backward rows: c1, -s1, c2, s2.
-// Lanes past rot turn by cosine 1, sine 0. The head rows' lanes share the work.
+// A warp's table of a token's rotation in shared memory, four rows of fp32 quads laid out
+// [row][quad][lane]: all its head rows use the same factors, so a lane reads them where it needs
+// them instead of holding 4 V registers. Forward rows: y1 = r (x1 A + x2 B), y2 = r (x2 C + x1 D)
+// with the weights inside (A = w1 c1, B = -w2 s1, C = w2 c2, D = w1 s2); backward rows: c1, -s1,
+// c2, s2. Lanes past rot turn by cosine 1, sine 0. The head rows' lanes share the work.
 template <int V, bool kWeights>
 __device__ __forceinline__ void make_table(float4 *tab, const float *cosv, const float *sinv,
                                            int64_t row, const float *w, const Lane<V> &ln,
@@ -310,7 +313,8 @@ __global__ void __launch_bounds__(kThreads, kFwdPerSm)
   ahead.tok = wk.tok;
   ahead.g = wk.part;
   auto locate = [&]() {
-    ahead.locate(dm, sp, wk, ln.slot, static_cast<const char *>(qkv), nullptr, nullptr, nullptr, es);
+    ahead.locate(dm, sp, wk, ln.slot, static_cast<const char *>(qkv), nullptr, nullptr, nullptr,
+                 es);
   };
   locate();
   auto fetch = [&](int stage) {
@@ -492,7 +496,8 @@ __global__ void __launch_bounds__(kThreads, kBwdPerSm)
         }
       }
       int left = n - (g - g0) * sp.at_once - ln.slot;
-      char *out = static_cast<char *>(dqkv) + (tok * total + first + (n - left)) * (int64_t)dm.d * es;
+      char *out =
+          static_cast<char *>(dqkv) + (tok * total + first + (n - left)) * (int64_t)dm.d * es;
       const char *lora =
           static_cast<const char *>(lq) + (tok * n + (n - left)) * (int64_t)dm.d * elem_size<L>();
       for (; g < g1; g += sp.parts) {
@@ -603,7 +608,8 @@ __global__ void __launch_bounds__(kThreads, kBwdPerSm)
   }
 }
 
-// Any even head size and alignment: a warp per head row, a lane per pair of dims at a time.
+// Any even head size and alignment: a warp per head row, a lane per pair of dims at a time (4096
+// tokens of 12 + 2 + 2 heads of 100, bf16: 41 us, issue 65 %, against 4 for its bytes).
 template <int T>
 __device__ __forceinline__ float load_x(const void *qkv, const void *l, int l_type, int64_t at,
                                         int64_t li, int i) {
@@ -638,7 +644,8 @@ __global__ void __launch_bounds__(256)
   pdl_release();
   const int lane = threadIdx.x & 31, total = dm.nh + 2 * dm.nkv;
   const int64_t n = dm.rows * total;
-  for (int64_t u = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); u < n; u += (int64_t)gridDim.x * 8) {
+  for (int64_t u = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); u < n;
+       u += (int64_t)gridDim.x * 8) {
     const int64_t tok = u / total;
     const int hr = (int)(u - tok * total);
     const int64_t pos = pos_idx[tok];
@@ -679,7 +686,8 @@ __global__ void __launch_bounds__(256)
 }
 
 // A CTA of one warp per token range; its dw sums live in shared memory, each element touched by
-// one lane only.
+// one lane only. The same tokens: 174 us (6 for the bytes), waiting for each load with 8 warps an
+// SM (issue 16 %, DRAM 2 %): for sizes and alignments that a training step does not have.
 template <int T>
 __global__ void __launch_bounds__(32)
     norm_rope_bwd_any(const void *dq, const void *dk, const void *dv, const void *qkv,
@@ -830,8 +838,9 @@ int check(const char *what, const NormDims &dm, int64_t batch, int64_t seq, int 
           int w_type) {
   if (dm.rows < 0 || batch < 0 || seq <= 0 || dm.nh <= 0 || dm.nkv < 0 || dm.d <= 0 || dm.d % 2 ||
       dm.rot < 0 || dm.rot % 2 || dm.rot > dm.d)
-    return set_error(TB_EINVAL, "%s: bad dims rows=%lld batch=%lld seq=%lld nh=%d nkv=%d d=%d rot=%d",
-                     what, (long long)dm.rows, (long long)batch, (long long)seq, dm.nh, dm.nkv,
+    return set_error(TB_EINVAL,
+                     "%s: bad dims rows=%lld batch=%lld seq=%lld nh=%d nkv=%d d=%d rot=%d", what,
+                     (long long)dm.rows, (long long)batch, (long long)seq, dm.nh, dm.nkv,
                      dm.d, dm.rot);
   if (dm.d > 4096 || dm.nh > 65536 || dm.nkv > 65536)
     return set_error(TB_EINVAL, "%s: head_dim %d (at most 4096), heads %d / %d (at most 65536)",
@@ -849,8 +858,9 @@ int check(const char *what, const NormDims &dm, int64_t batch, int64_t seq, int 
 // Shared memory beyond 48 KB has to be asked for, on every device.
 template <typename Kernel>
 int allow_smem(const char *what, Kernel kernel, size_t bytes) {
-  if (bytes <= 48 * 1024 || cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 (int)bytes) == cudaSuccess)
+  if (bytes <= 48 * 1024 ||
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) ==
+          cudaSuccess)
     return TB_OK;
   (void)cudaGetLastError();
   return set_error(TB_ELAUNCH, "%s: %d bytes of shared memory", what, (int)bytes);

@@ -71,9 +71,10 @@ class NormRopeTokens(torch.autograd.Function):
             ws = cos.new_empty(max(nbytes // 4, 1))
         _lib.call_on(qkv, "tb_norm_rope_bwd", *(_lib.addr(g) for g in grads), qkv.data_ptr(), code,
                      _ld(qkv), _lib.addr(lora_q), _code(lora_q, code), _lib.addr(q_weight),
-                     _lib.addr(k_weight), _code(q_weight if q_weight is not None else k_weight, code),
-                     weight_offset, eps, cos.data_ptr(), sin.data_ptr(), cos.shape[1],
-                     pos_idx.data_ptr(), dqkv.data_ptr(), _lib.addr(dqw), _lib.addr(dkw),
+                     _lib.addr(k_weight),
+                     _code(q_weight if q_weight is not None else k_weight, code), weight_offset,
+                     eps, cos.data_ptr(), sin.data_ptr(), cos.shape[1], pos_idx.data_ptr(),
+                     dqkv.data_ptr(), _lib.addr(dqw), _lib.addr(dkw),
                      _lib.addr(ws), nbytes, rows, batch, seq, n_heads, n_kv, head_dim)
         q_cols, v_start = n_heads * head_dim, (n_heads + n_kv) * head_dim
         return (dqkv if need[0] else None, dqkv[:, :q_cols] if need[1] else None,
@@ -105,9 +106,9 @@ def norm_rope_tokens(qkv, lora_q, lora_v, q_weight, k_weight, eps, cos, sin, pos
     `cos`, `sin` [>= seq, rot] with rot <= head_dim; a token's table row is pos_idx % seq, and one
     whose pos_idx is outside [0, batch * seq) gets zero rows and no gradient. qkv's rows may be
     views of wider rows; in 16-bit types rows that do not start on 16 bytes are several times slower
-    than a contiguous copy. Differentiable in qkv, lora_q, lora_v, q_weight and k_weight. Gradients of
-    the LoRA rows are qkv's gradient's columns, as in rope.rope_tokens: fp32 rows beside 16-bit qkv get
-    values rounded to qkv's type (beside fp16, 0 below 3e-8 and infinite above 65504)."""
+    than a contiguous copy. Differentiable in qkv, lora_q, lora_v, q_weight and k_weight. Gradients
+    of the LoRA rows are qkv's gradient's columns, as in rope.rope_tokens: fp32 rows beside 16-bit
+    qkv get values rounded to qkv's type (beside fp16, 0 below 3e-8 and infinite above 65504)."""
     _lib.require_cuda(qkv, lora_q, lora_v, q_weight, k_weight, cos, sin, pos_idx,
                       what="norm_rope_tokens")
     dtype, rows = qkv.dtype, qkv.shape[0] if qkv.dim() else 0
